@@ -1,4 +1,5 @@
-"""ctypes binding of ``libcruise_epoch.so`` (the C ABI in include/cruise_epoch.h).
+"""ctypes binding of ``libcruise_epoch.so`` (the C ABI in include/cruise_epoch.h
+and include/cruise_decoder.h).
 
 The library is built in-tree by :mod:`cruise_b200.build`.  There is no
 fallback: if the shared library is missing or fails to load, every engine
@@ -20,6 +21,7 @@ i32p = ctypes.POINTER(ctypes.c_int32)
 i64p = ctypes.POINTER(ctypes.c_int64)
 u8p = ctypes.POINTER(ctypes.c_uint8)
 f32p = ctypes.POINTER(ctypes.c_float)
+_ptr, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 
 # symbol -> (restype, argtypes); the exported surface of include/cruise_epoch.h
 SIGNATURES = {
@@ -96,6 +98,24 @@ SIGNATURES = {
     "cruise_epoch_stream_enable": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_int32]),
     "cruise_epoch_stream_next_id": (ctypes.c_uint32, [ctypes.c_void_p]),
     "cruise_epoch_stream_poll": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p]),
+    # include/cruise_decoder.h: pointers are device addresses (ints, None for NULL)
+    "cruise_decoder_rotate_store": (
+        ctypes.c_int32,
+        [_ptr, _i64, _i32, _i32, _i32, _i32, _i32, _ptr, _ptr, _ptr, _ptr, _f32, _ptr, _ptr, _i32, _i32, _i32, _ptr,
+         _i64, _ptr, _ptr, _i64, _i32, _i64, _i32, _ptr],
+    ),
+    "cruise_decoder_attention": (
+        ctypes.c_int32,
+        [_ptr, _i64, _i32, _i32, _i32, _i32, _i32, _ptr, _ptr, _i64, _i32, _i64, _ptr, _i64, _i32, _ptr, _f32, _ptr,
+         _i64, _ptr, _ptr, _i64, _i32, _ptr],
+    ),
+    "cruise_decoder_attention_workspace": (ctypes.c_int64, [_i32, _i32, _i32, _i32, _i64, _i32]),
+    "cruise_decoder_choose": (
+        ctypes.c_int32,
+        [_ptr, _i64, _i32, _i32, _i32, _ptr, _ptr, _i64, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i32,
+         _ptr, _ptr, _i64, _ptr, _i64, _ptr, _i32, _i32, _ptr],
+    ),
+    "cruise_decoder_last_error": (ctypes.c_char_p, []),
 }
 
 _LIB: ctypes.CDLL | None = None

@@ -18,7 +18,7 @@ PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE / "csrc"
 LIBRARY = PACKAGE / "libcruise_epoch.so"
 SERVER = PACKAGE / "cruise_epoch_server"
-SOURCES = [CSRC / "engine.cu"]
+SOURCES = [CSRC / "engine.cu", CSRC / "decoder_ops.cu"]
 SERVER_SOURCES = [CSRC / "sidecar_server.cpp"]
 HEADERS = list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list((PACKAGE.parent / "include").glob("*.h"))
 NVCC_FLAGS = [

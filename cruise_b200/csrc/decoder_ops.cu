@@ -1,0 +1,437 @@
+// decoder_ops.cu -- launches and C ABI of the decoder operators
+// (include/cruise_decoder.h).
+#include <algorithm>
+#include <atomic>
+#include <cstdarg>
+#include <cstdio>
+
+#include "../../include/cruise_decoder.h"
+#include "decoder_attention.cuh"
+#include "decoder_choose.cuh"
+#include "decoder_ops.h"
+#include "decoder_rotate.cuh"
+
+namespace cruise {
+namespace ops {
+namespace {
+
+constexpr int kMaxDevices = 64;
+constexpr int64_t kMaxIndex = 0x7fffffff;
+
+// Streaming multiprocessors of a device (148 where it cannot be asked: sizes
+// are then only planned, not run).
+int sm_count(int device) {
+  static std::atomic<int> known[kMaxDevices];
+  const bool cached = device >= 0 && device < kMaxDevices;
+  if (cached) {
+    const int n = known[device].load(std::memory_order_relaxed);
+    if (n > 0) return n;
+  }
+  int n = 0;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    return 148;
+  }
+  if (cached) known[device].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// The calling thread's device for the length of a launch.
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device) {
+    error = cudaGetDevice(&before_);
+    if (error == cudaSuccess && before_ != device) {
+      error = cudaSetDevice(device);
+      moved_ = error == cudaSuccess;
+    }
+  }
+  ~DeviceScope() {
+    if (moved_) cudaSetDevice(before_);
+  }
+  cudaError_t error = cudaSuccess;
+
+ private:
+  int before_ = 0;
+  bool moved_ = false;
+};
+
+// Raises a kernel's shared-memory limit once per device.
+template <typename Kernel>
+cudaError_t allow_shared(Kernel kernel, size_t bytes, int device, std::atomic<uint64_t> &done, bool wide_cluster = false) {
+  const uint64_t bit = device >= 0 && device < kMaxDevices ? 1ull << device : 0;
+  if (bit != 0 && (done.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (err == cudaSuccess && wide_cluster)
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return err;
+}
+
+// ---- rotate_store --------------------------------------------------------------
+
+template <typename T, int D>
+cudaError_t rotate_typed(const RotateArgs &a, int device, cudaStream_t stream) {
+  constexpr int kHeads = 256 / D;   // heads a warp moves per round
+  const int all = (a.nq + 2 * a.nkv + kHeads - 1) / kHeads;
+  // as many rounds per warp as still leave 16 warps per SM: few tokens spread
+  // their heads over the GPU, many keep their table row in registers
+  const int64_t want = static_cast<int64_t>(sm_count(device)) * 16;
+  const int rounds = static_cast<int>(std::clamp<int64_t>(static_cast<int64_t>(a.tokens) * all / want, 1, all));
+  const int warps_per_token = (all + rounds - 1) / rounds;
+  const int64_t warps = static_cast<int64_t>(a.tokens) * warps_per_token;
+  const unsigned grid = static_cast<unsigned>((warps * 32 + kRotateThreads - 1) / kRotateThreads);
+  rotate_store_kernel<T, D><<<grid, kRotateThreads, 0, stream>>>(a, rounds, warps_per_token);
+  return cudaGetLastError();
+}
+
+// ---- paged_attention -----------------------------------------------------------
+
+// How the heads of a KV head form units of at most 16, and whether a unit is
+// worth splitting over the length.
+struct AttentionShape {
+  int32_t groups, chunks, chunk, units;
+  bool whole;
+  int grid;   // CTAs of the split form
+};
+
+AttentionShape attention_shape(int32_t rows, int32_t nq, int32_t nkv, int64_t capacity, int device) {
+  AttentionShape s;
+  s.groups = nq / nkv;
+  s.chunks = (s.groups + 15) / 16;
+  s.chunk = (s.groups + s.chunks - 1) / s.chunks;
+  s.units = nkv * s.chunks;
+  s.whole = capacity <= 8 * kAttendTile;
+  s.grid = sm_count(device) * kAttendCtas;
+  (void)rows;
+  return s;
+}
+
+size_t align16(size_t v) { return (v + 15) / 16 * 16; }
+
+size_t pieces_bytes(int grid, int heads, int d, size_t *ml, size_t *of) {
+  size_t bytes = align16(static_cast<size_t>(2) * grid * heads * d * 4);
+  if (ml != nullptr) *ml = bytes;
+  bytes += align16(static_cast<size_t>(2) * grid * heads * 2 * 4);
+  if (of != nullptr) *of = bytes;
+  return bytes + static_cast<size_t>(grid) * sizeof(int4);
+}
+
+template <typename T, int D, int NT>
+cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int device, cudaStream_t stream) {
+  AttentionPlan p{};
+  p.a = a;
+  p.groups = s.groups;
+  p.chunk = s.chunk;
+  p.chunks = s.chunks;
+  p.units = s.units;
+  p.block_shift = -1;
+  for (int b = 0; b < 31; ++b)
+    if (a.block_size == 1 << b) p.block_shift = b;
+  p.capacity = a.table_width * a.block_size;
+  p.whole = s.whole ? 1 : 0;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  if (!s.whole) {
+    size_t ml = 0, of = 0;
+    pieces_bytes(s.grid, NT * 8, D, &ml, &of);
+    uint8_t *w = static_cast<uint8_t *>(a.workspace);
+    p.piece_o = reinterpret_cast<float *>(w);
+    p.piece_ml = reinterpret_cast<float *>(w + ml);
+    p.piece_of = reinterpret_cast<int4 *>(w + of);
+  }
+  static std::atomic<uint64_t> done{0};
+  constexpr size_t smem = AttendShared<D>::kRingBytes;
+  cudaError_t err = allow_shared(attention_kernel<T, D, NT>, smem, device, done);
+  if (err != cudaSuccess) return err;
+  const unsigned grid = s.whole ? static_cast<unsigned>(a.rows) * s.units : static_cast<unsigned>(s.grid);
+  attention_kernel<T, D, NT><<<grid, kAttendThreads, smem, stream>>>(p);
+  err = cudaGetLastError();
+  if (err != cudaSuccess || s.whole) return err;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(s.grid, s.chunk);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attention_join_kernel<T, D, NT>, p);
+}
+
+template <typename T>
+cudaError_t attention_of(const AttentionArgs &a, const AttentionShape &s, int device, cudaStream_t stream) {
+  if (a.d == 128)
+    return s.chunk <= 8 ? attention_typed<T, 128, 1>(a, s, device, stream) : attention_typed<T, 128, 2>(a, s, device, stream);
+  return s.chunk <= 8 ? attention_typed<T, 64, 1>(a, s, device, stream) : attention_typed<T, 64, 2>(a, s, device, stream);
+}
+
+// ---- choose --------------------------------------------------------------------
+
+template <typename T>
+cudaError_t choose_typed(const ChooseArgs &a, int device, cudaStream_t stream) {
+  // CTAs per row: enough for two per SM, each with a slice whose words fit
+  // three CTAs to an SM where possible
+  const int64_t want = 2ll * sm_count(device);
+  int ctas = 1;
+  while (ctas < kChooseMaxCluster && (static_cast<int64_t>(a.rows) * ctas < want || choose_slice(a.vocab, ctas) > 18 * 1024) &&
+         choose_slice(a.vocab, ctas) > 1024)
+    ctas *= 2;
+  const size_t smem = static_cast<size_t>(choose_slice(a.vocab, ctas)) * 4;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t err = allow_shared(choose_kernel<T>, 200 * 1024, device, done, true);
+  if (err != cudaSuccess) return err;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.gridDim = dim3(ctas, a.rows);
+  cfg.blockDim = dim3(kChooseThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, choose_kernel<T>, a);
+}
+
+// ---- errors --------------------------------------------------------------------
+
+thread_local char g_error[256] = "";
+
+int32_t refuse(const char *format, ...) {
+  va_list args;
+  va_start(args, format);
+  std::vsnprintf(g_error, sizeof(g_error), format, args);
+  va_end(args);
+  return -1;
+}
+
+int32_t report(cudaError_t err, const char *what) {
+  if (err == cudaSuccess) {
+    g_error[0] = 0;
+    return 0;
+  }
+  std::snprintf(g_error, sizeof(g_error), "%s: %s", what, cudaGetErrorString(err));
+  return static_cast<int32_t>(err);
+}
+
+bool aligned(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// Whether [a, a + na) and [b, b + nb) bytes overlap.
+bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na > 0 && nb > 0 && x < y + static_cast<uintptr_t>(nb) && y < x + static_cast<uintptr_t>(na);
+}
+
+int64_t extent(int64_t rows, int64_t stride, int64_t width, int64_t size) {
+  return rows > 0 ? ((rows - 1) * stride + width) * size : 0;
+}
+
+}  // namespace
+
+cudaError_t launch_rotate_store(const RotateArgs &a, int device, cudaStream_t stream) {
+  if (a.tokens == 0) return cudaSuccess;
+  if (a.dtype == kBf16)
+    return a.d == 128 ? rotate_typed<__nv_bfloat16, 128>(a, device, stream) : rotate_typed<__nv_bfloat16, 64>(a, device, stream);
+  return a.d == 128 ? rotate_typed<__half, 128>(a, device, stream) : rotate_typed<__half, 64>(a, device, stream);
+}
+
+int64_t attention_workspace(int32_t rows, int32_t nq, int32_t nkv, int32_t d, int64_t capacity, int device) {
+  const AttentionShape s = attention_shape(rows, nq, nkv, capacity, device);
+  if (s.whole) return 0;
+  return static_cast<int64_t>(pieces_bytes(s.grid, s.chunk <= 8 ? 8 : 16, d, nullptr, nullptr));
+}
+
+cudaError_t launch_paged_attention(const AttentionArgs &a, int device, cudaStream_t stream) {
+  if (a.rows == 0) return cudaSuccess;
+  const AttentionShape s =
+      attention_shape(a.rows, a.nq, a.nkv, static_cast<int64_t>(a.table_width) * a.block_size, device);
+  return a.dtype == kBf16 ? attention_of<__nv_bfloat16>(a, s, device, stream) : attention_of<__half>(a, s, device, stream);
+}
+
+cudaError_t launch_choose(const ChooseArgs &a, int device, cudaStream_t stream) {
+  if (a.rows == 0) return cudaSuccess;
+  switch (a.dtype) {
+    case kFp32: return choose_typed<float>(a, device, stream);
+    case kBf16: return choose_typed<__nv_bfloat16>(a, device, stream);
+    default: return choose_typed<__half>(a, device, stream);
+  }
+}
+
+}  // namespace ops
+}  // namespace cruise
+
+using namespace cruise::ops;
+
+extern "C" {
+
+const char *cruise_decoder_last_error(void) { return g_error; }
+
+int32_t cruise_decoder_rotate_store(const void *qkv, int64_t qkv_stride, int32_t tokens, int32_t num_heads,
+                                    int32_t num_kv_heads, int32_t head_dim, int32_t dtype, const int64_t *position,
+                                    const int32_t *slot, const void *q_norm, const void *k_norm, float eps,
+                                    const void *rope_cos, const void *rope_sin, int32_t rope_dtype, int32_t rope_rows,
+                                    int32_t rotary, void *q_out, int64_t q_stride, void *key_cache, void *value_cache,
+                                    int64_t num_blocks, int32_t block_size, int64_t block_stride, int32_t device,
+                                    void *stream) {
+  const char *const op = "cruise_decoder_rotate_store";
+  if (tokens < 0 || num_heads < 1 || num_kv_heads < 1 || num_heads > 1024 || num_kv_heads > 1024)
+    return refuse("%s: %d tokens of %d query and %d KV heads (tokens >= 0, heads 1 to 1024)", op, tokens, num_heads, num_kv_heads);
+  if (head_dim != 64 && head_dim != 128) return refuse("%s: head size %d (64 or 128)", op, head_dim);
+  if (dtype != kBf16 && dtype != kFp16) return refuse("%s: dtype %d (0 bf16 or 1 fp16)", op, dtype);
+  if (rope_dtype != kBf16 && rope_dtype != kFp32) return refuse("%s: rope dtype %d (0 bf16 or 2 fp32)", op, rope_dtype);
+  if (rope_rows < 1 || rotary < 16 || rotary % 16 != 0 || rotary > head_dim)
+    return refuse("%s: tables of %d rows x %d (rows >= 1, a multiple of 16 up to the head size)", op, rope_rows, rotary);
+  if ((q_norm == nullptr) != (k_norm == nullptr)) return refuse("%s: pass both norm weights or neither", op);
+  if (num_blocks < 1 || block_size < 1 || num_blocks > kMaxIndex / block_size)
+    return refuse("%s: a cache of %lld blocks of %d slots (at least one, slots below 2^31)", op, static_cast<long long>(num_blocks), block_size);
+  const int64_t width = static_cast<int64_t>(num_heads + 2 * num_kv_heads) * head_dim, q_width = static_cast<int64_t>(num_heads) * head_dim;
+  const int64_t block_elems = static_cast<int64_t>(block_size) * num_kv_heads * head_dim;
+  if (qkv_stride < width || q_stride < q_width || block_stride < block_elems)
+    return refuse("%s: a stride is smaller than its row (qkv %lld, q %lld, block %lld)", op, static_cast<long long>(qkv_stride),
+                  static_cast<long long>(q_stride), static_cast<long long>(block_stride));
+  if (qkv_stride % 8 != 0 || q_stride % 8 != 0 || block_stride % 8 != 0)
+    return refuse("%s: strides must be multiples of 8 elements", op);
+  if (tokens == 0) return report(cudaSuccess, op);
+  if (qkv == nullptr || position == nullptr || slot == nullptr || rope_cos == nullptr || rope_sin == nullptr ||
+      q_out == nullptr || key_cache == nullptr || value_cache == nullptr)
+    return refuse("%s: a required pointer is NULL", op);
+  if (!aligned(qkv, 16) || !aligned(q_norm, 16) || !aligned(k_norm, 16) || !aligned(rope_cos, 16) ||
+      !aligned(rope_sin, 16) || !aligned(q_out, 16) || !aligned(key_cache, 16) || !aligned(value_cache, 16) ||
+      !aligned(position, 8) || !aligned(slot, 4))
+    return refuse("%s: pointers must be 16-byte aligned (position 8, slot 4)", op);
+  const int64_t in_bytes = extent(tokens, qkv_stride, width, 2), out_bytes = extent(tokens, q_stride, q_width, 2);
+  const int64_t cache_bytes = extent(num_blocks, block_stride, block_elems, 2);
+  if (overlap(q_out, out_bytes, qkv, in_bytes) || overlap(key_cache, cache_bytes, qkv, in_bytes) ||
+      overlap(value_cache, cache_bytes, qkv, in_bytes) || overlap(q_out, out_bytes, key_cache, cache_bytes) ||
+      overlap(q_out, out_bytes, value_cache, cache_bytes))
+    return refuse("%s: q_out, the caches and qkv must not overlap", op);
+  DeviceScope scope(device);
+  if (scope.error != cudaSuccess) return report(scope.error, op);
+  RotateArgs a{qkv, qkv_stride, tokens, num_heads, num_kv_heads, head_dim, dtype, position, slot, q_norm, k_norm, eps,
+               rope_cos, rope_sin, rope_dtype, rope_rows, rotary, q_out, q_stride, key_cache, value_cache, num_blocks,
+               block_stride, block_size};
+  return report(launch_rotate_store(a, device, static_cast<cudaStream_t>(stream)), op);
+}
+
+static int32_t check_attention_sizes(const char *op, int32_t rows, int32_t num_heads, int32_t num_kv_heads,
+                                     int32_t head_dim, int64_t capacity) {
+  if (rows < 0 || num_kv_heads < 1 || num_heads < 1 || num_heads % num_kv_heads != 0 || num_heads > 1024)
+    return refuse("%s: %d rows of %d query heads over %d KV heads (a multiple, at most 1024)", op, rows, num_heads, num_kv_heads);
+  if (head_dim != 64 && head_dim != 128) return refuse("%s: head size %d (64 or 128)", op, head_dim);
+  if (capacity < 0 || capacity > kMaxIndex - kAttendTile) return refuse("%s: a capacity of %lld positions (below 2^31)", op, static_cast<long long>(capacity));
+  const int64_t units = static_cast<int64_t>(num_kv_heads) * ((num_heads / num_kv_heads + 15) / 16);
+  if (rows * units * std::max<int64_t>(1, (capacity + kAttendTile - 1) / kAttendTile) > kMaxIndex)
+    return refuse("%s: rows x KV heads x capacity / %d passes 2^31", op, kAttendTile);
+  return 0;
+}
+
+int64_t cruise_decoder_attention_workspace(int32_t rows, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                           int64_t capacity, int32_t device) {
+  const char *const op = "cruise_decoder_attention_workspace";
+  if (check_attention_sizes(op, rows, num_heads, num_kv_heads, head_dim, capacity) != 0) return -1;
+  report(cudaSuccess, op);
+  return attention_workspace(rows, num_heads, num_kv_heads, head_dim, capacity, device);
+}
+
+int32_t cruise_decoder_attention(const void *q, int64_t q_stride, int32_t rows, int32_t num_heads, int32_t num_kv_heads,
+                                 int32_t head_dim, int32_t dtype, const void *key_cache, const void *value_cache,
+                                 int64_t num_blocks, int32_t block_size, int64_t block_stride,
+                                 const int32_t *block_table, int64_t table_stride, int32_t table_width,
+                                 const int32_t *seq_len, float scale, void *out, int64_t out_stride, float *lse,
+                                 void *workspace, int64_t workspace_bytes, int32_t device, void *stream) {
+  const char *const op = "cruise_decoder_attention";
+  if (dtype != kBf16 && dtype != kFp16) return refuse("%s: dtype %d (0 bf16 or 1 fp16)", op, dtype);
+  if (num_blocks < 1 || block_size < 1 || table_width < 0 || num_blocks > kMaxIndex / block_size)
+    return refuse("%s: a cache of %lld blocks of %d slots, tables of %d (at least one block, slots below 2^31)", op,
+                  static_cast<long long>(num_blocks), block_size, table_width);
+  const int64_t capacity = static_cast<int64_t>(table_width) * block_size;
+  if (const int32_t bad = check_attention_sizes(op, rows, num_heads, num_kv_heads, head_dim, capacity)) return bad;
+  const int64_t width = static_cast<int64_t>(num_heads) * head_dim;
+  const int64_t block_elems = static_cast<int64_t>(block_size) * num_kv_heads * head_dim;
+  if (q_stride < width || out_stride < width || block_stride < block_elems || table_stride < table_width)
+    return refuse("%s: a stride is smaller than its row (q %lld, out %lld, block %lld, table %lld)", op,
+                  static_cast<long long>(q_stride), static_cast<long long>(out_stride), static_cast<long long>(block_stride),
+                  static_cast<long long>(table_stride));
+  if (q_stride % 8 != 0 || out_stride % 8 != 0 || block_stride % 8 != 0)
+    return refuse("%s: strides must be multiples of 8 elements", op);
+  if (!(scale - scale == 0.f)) return refuse("%s: the scale must be finite", op);
+  if (rows == 0) return report(cudaSuccess, op);
+  if (q == nullptr || key_cache == nullptr || value_cache == nullptr || seq_len == nullptr || out == nullptr ||
+      (block_table == nullptr && table_width > 0))
+    return refuse("%s: a required pointer is NULL", op);
+  if (!aligned(q, 16) || !aligned(key_cache, 16) || !aligned(value_cache, 16) || !aligned(out, 16) ||
+      !aligned(workspace, 16) || !aligned(block_table, 4) || !aligned(seq_len, 4) || !aligned(lse, 4))
+    return refuse("%s: pointers must be 16-byte aligned (block_table, seq_len, lse 4)", op);
+  const int64_t out_bytes = extent(rows, out_stride, width, 2), lse_bytes = lse != nullptr ? 4ll * rows * num_heads : 0;
+  const int64_t cache_bytes = extent(num_blocks, block_stride, block_elems, 2), q_bytes = extent(rows, q_stride, width, 2);
+  const int64_t table_bytes = extent(rows, table_stride, table_width, 4);
+  if (overlap(out, out_bytes, q, q_bytes) || overlap(out, out_bytes, key_cache, cache_bytes) ||
+      overlap(out, out_bytes, value_cache, cache_bytes) || overlap(out, out_bytes, block_table, table_bytes) ||
+      overlap(out, out_bytes, seq_len, 4ll * rows) || overlap(lse, lse_bytes, out, out_bytes) ||
+      overlap(lse, lse_bytes, q, q_bytes) || overlap(lse, lse_bytes, key_cache, cache_bytes) ||
+      overlap(lse, lse_bytes, value_cache, cache_bytes) || overlap(lse, lse_bytes, block_table, table_bytes) ||
+      overlap(lse, lse_bytes, seq_len, 4ll * rows))
+    return refuse("%s: out and lse must not overlap the inputs or each other", op);
+  DeviceScope scope(device);
+  if (scope.error != cudaSuccess) return report(scope.error, op);
+  const int64_t need = attention_workspace(rows, num_heads, num_kv_heads, head_dim, capacity, device);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return refuse("%s: a workspace of %lld bytes, %lld needed", op, static_cast<long long>(workspace != nullptr ? workspace_bytes : 0),
+                  static_cast<long long>(need));
+  if (need > 0 && (overlap(workspace, need, out, out_bytes) || overlap(workspace, need, lse, lse_bytes) ||
+                   overlap(workspace, need, q, q_bytes) || overlap(workspace, need, key_cache, cache_bytes) ||
+                   overlap(workspace, need, value_cache, cache_bytes) || overlap(workspace, need, block_table, table_bytes) ||
+                   overlap(workspace, need, seq_len, 4ll * rows)))
+    return refuse("%s: the workspace must not overlap the tensors", op);
+  AttentionArgs a{q, q_stride, rows, num_heads, num_kv_heads, head_dim, dtype, key_cache, value_cache, num_blocks,
+                  block_stride, block_size, block_table, table_stride, table_width, seq_len, scale, out, out_stride, lse,
+                  workspace};
+  return report(launch_paged_attention(a, device, static_cast<cudaStream_t>(stream)), op);
+}
+
+int32_t cruise_decoder_choose(const void *logits, int64_t logits_stride, int32_t rows, int32_t vocab, int32_t dtype,
+                              const int32_t *active, int32_t *history, int64_t history_stride, int32_t history_width,
+                              const int32_t *prompt_len, const int32_t *history_len, const float *repetition,
+                              const float *frequency, const float *presence, const int32_t *bias_token,
+                              const float *bias_value, int64_t bias_stride, int32_t bias_width, const int32_t *bias_len,
+                              const uint32_t *allowed, int64_t allowed_stride, float *processed,
+                              int64_t processed_stride, int64_t *token, int32_t append, int32_t device, void *stream) {
+  const char *const op = "cruise_decoder_choose";
+  if (rows < 0 || rows > 65535 || vocab < 1 || vocab > 800000)
+    return refuse("%s: %d rows of %d logits (at most 65535 rows of 1 to 800000)", op, rows, vocab);
+  if (dtype < kBf16 || dtype > kFp32) return refuse("%s: dtype %d (0 bf16, 1 fp16 or 2 fp32)", op, dtype);
+  if (logits_stride < vocab || (processed != nullptr && processed_stride < vocab) ||
+      (allowed != nullptr && allowed_stride < (vocab + 31) / 32))
+    return refuse("%s: a stride is smaller than its row", op);
+  if (history != nullptr && (history_width < 1 || history_stride < history_width || prompt_len == nullptr || history_len == nullptr))
+    return refuse("%s: a history needs a width (at most its stride), prompt_len and history_len", op);
+  if (history == nullptr && (append != 0 || repetition != nullptr || frequency != nullptr || presence != nullptr))
+    return refuse("%s: penalties and append need a history", op);
+  if (bias_token != nullptr && (bias_width < 1 || bias_stride < bias_width || bias_value == nullptr || bias_len == nullptr))
+    return refuse("%s: a bias list needs a width (at most its stride), bias_value and bias_len", op);
+  if (rows == 0) return report(cudaSuccess, op);
+  if (logits == nullptr || token == nullptr) return refuse("%s: a required pointer is NULL", op);
+  const int size = dtype == kFp32 ? 4 : 2;
+  if (!aligned(logits, size) || !aligned(token, 8) || !aligned(active, 4) || !aligned(history, 4) ||
+      !aligned(prompt_len, 4) || !aligned(history_len, 4) || !aligned(repetition, 4) || !aligned(frequency, 4) ||
+      !aligned(presence, 4) || !aligned(bias_token, 4) || !aligned(bias_value, 4) || !aligned(bias_len, 4) ||
+      !aligned(allowed, 4) || !aligned(processed, 4))
+    return refuse("%s: a pointer is not aligned to its element", op);
+  const int64_t logits_bytes = extent(rows, logits_stride, vocab, size);
+  if (processed != nullptr) {
+    const bool in_place = static_cast<const void *>(processed) == logits && dtype == kFp32 && processed_stride == logits_stride;
+    if (!in_place && overlap(processed, extent(rows, processed_stride, vocab, 4), logits, logits_bytes))
+      return refuse("%s: processed must be the fp32 logits themselves or not overlap them", op);
+  }
+  DeviceScope scope(device);
+  if (scope.error != cudaSuccess) return report(scope.error, op);
+  ChooseArgs a{logits, logits_stride, rows, vocab, dtype, active, history, history_stride, history_width, prompt_len,
+               history_len, repetition, frequency, presence, bias_token, bias_value, bias_stride, bias_width, bias_len,
+               allowed, allowed_stride, processed, processed_stride, token, append != 0 ? 1 : 0};
+  return report(launch_choose(a, device, static_cast<cudaStream_t>(stream)), op);
+}
+
+}  // extern "C"
