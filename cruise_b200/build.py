@@ -1,8 +1,9 @@
-"""Builds the engine's shared library in-tree with nvcc for sm_100a, and the
-sidecar server (a plain C++ program over the library's C ABI).
+"""Builds the engine's shared library in-tree with nvcc for sm_100a, the sidecar
+server (a plain C++ program over the library's C ABI) and the Python calls of
+the decoder operators (an extension module against torch's headers).
 
-``python -m cruise_b200.build`` writes ``cruise_b200/libcruise_epoch.so`` and
-``cruise_b200/cruise_epoch_server``.  nvcc cross-compiles without a GPU, so this
+``python -m cruise_b200.build`` writes ``cruise_b200/libcruise_epoch.so``,
+``cruise_b200/cruise_epoch_server`` and ``cruise_b200/_decoder_bind.so``.  nvcc cross-compiles without a GPU, so this
 runs on any host with CUDA 12.9.
 """
 
@@ -20,6 +21,8 @@ LIBRARY = PACKAGE / "libcruise_epoch.so"
 SERVER = PACKAGE / "cruise_epoch_server"
 SOURCES = [CSRC / "engine.cu", CSRC / "decoder_ops.cu"]
 SERVER_SOURCES = [CSRC / "sidecar_server.cpp"]
+BINDING = PACKAGE / "_decoder_bind.so"
+BINDING_SOURCES = [CSRC / "decoder_bind.cpp"]
 HEADERS = list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list((PACKAGE.parent / "include").glob("*.h"))
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -42,7 +45,8 @@ def _fresh(target: Path, sources: list[Path]) -> bool:
 
 
 def up_to_date() -> bool:
-    return _fresh(LIBRARY, SOURCES) and _fresh(SERVER, SERVER_SOURCES + [LIBRARY])
+    return (_fresh(LIBRARY, SOURCES) and _fresh(SERVER, SERVER_SOURCES + [LIBRARY])
+            and _fresh(BINDING, BINDING_SOURCES))
 
 
 def build_server() -> Path:
@@ -56,6 +60,27 @@ def build_server() -> Path:
     subprocess.run(cmd, check=True)
     os.replace(tmp, SERVER)
     return SERVER
+
+
+def build_binding() -> Path:
+    """The Python calls of the decoder operators (cruise_b200._decoder_bind)."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("a C++ compiler (g++) is required to build the decoder operators' Python calls")
+    cuda = str(Path(nvcc()).resolve().parents[1] / "include")
+    tmp = BINDING.with_name(f"{BINDING.name}.tmp{os.getpid()}")
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", sysconfig.get_paths()["include"], *(arg for path in [*include_paths(), cuda] for arg in ("-isystem", path)),
+           "-o", str(tmp), *map(str, BINDING_SOURCES), *(f"-L{path}" for path in library_paths()),
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, BINDING)
+    return BINDING
 
 
 def link_flags() -> list[str]:
@@ -74,6 +99,8 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         subprocess.run(cmd, check=True)
         os.replace(tmp, LIBRARY)
     build_server()
+    if force or not _fresh(BINDING, BINDING_SOURCES):
+        build_binding()
     return LIBRARY
 
 

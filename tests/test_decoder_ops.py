@@ -4,8 +4,6 @@ Python calls before the library."""
 
 from __future__ import annotations
 
-import ctypes
-
 import pytest
 import torch
 
@@ -131,11 +129,16 @@ def test_python_calls_refuse_cpu_tensors():
         decoder_ops.choose([[0.0]])
 
 
-def test_statuses_become_exceptions():
-    _lib.load().cruise_decoder_choose(*{**CHOOSE, "vocab": 0}.values())
-    with pytest.raises(ValueError, match="logits"):
-        decoder_ops._done(-1)
-    with pytest.raises(decoder_ops.DecoderOpError) as err:
-        decoder_ops._done(700)
-    assert err.value.code == 700 and isinstance(err.value, RuntimeError)
-    assert ctypes.c_char_p is _lib.SIGNATURES["cruise_decoder_last_error"][0]
+def test_a_cuda_failure_is_an_exception_with_its_code():
+    error = decoder_ops.DecoderOpError(700, "why")
+    assert error.code == 700 and isinstance(error, RuntimeError) and "why" in str(error)
+
+
+def test_the_python_calls_use_the_loaded_library():
+    assert decoder_ops._bind.bind is not None
+    with pytest.raises(ValueError, match="NULL"):
+        decoder_ops._bind.bind(0, 0, 0, 0, 0, RuntimeError)
+    with pytest.raises(TypeError, match="arguments"):
+        decoder_ops._bind.choose(1, 2)
+    with pytest.raises(ValueError, match="logits must be a CUDA tensor"):   # still bound
+        decoder_ops.choose(torch.zeros(1, 1))
