@@ -20,14 +20,20 @@
 namespace cruise {
 namespace ops {
 
-constexpr int kAttendWarps = 4;
-constexpr int kAttendThreads = kAttendWarps * 32;
-constexpr int kAttendKeys = 16;                          // keys of a warp's step
-constexpr int kAttendTile = kAttendWarps * kAttendKeys;  // keys of a CTA's step
+constexpr int kAttendKeys = 16;      // keys of a warp's step
 constexpr int kAttendStages = 3;
-constexpr int kAttendCtas = 2;                           // CTAs per SM
-constexpr int kAttendMinShare = 2;                       // fewest tiles worth a CTA of their own
-constexpr int kJoinThreads = 128;
+constexpr int kAttendWarps = 4;      // warps of a CTA that shares the work with the others
+constexpr int kAttendWholeWarps = 8; // warps of a CTA that takes one whole unit
+constexpr int kJoinThreads = 1024;
+constexpr int kJoinBatch = 6;        // pieces a thread has in flight
+
+// CTAs per SM that share the work: what shared memory (head size 128) or
+// registers allow.
+__host__ __device__ constexpr int attend_ctas(int d, int nt) { return d == 128 ? 2 : nt == 1 ? 4 : 3; }
+
+// What starting a unit costs, in tiles: the pipeline fills and the warps' parts
+// meet once per unit, whatever its length.
+__host__ __device__ constexpr int attend_setup(int d) { return d == 128 ? 2 : 4; }
 
 // Pieces of split units: CTA c leaves its first piece (of a unit that began
 // before c) in slot 2c and its last (of a unit that goes on after c) in 2c + 1.
@@ -39,18 +45,17 @@ struct AttentionPlan {
   int32_t units;       // units per row: nkv * chunks
   int32_t block_shift; // log2(block_size), -1 when not a power of two
   int32_t capacity;    // table_width * block_size
-  int32_t whole;       // 1: one CTA per unit, nothing to join
   float scale_log2;    // scale * log2(e)
   float *piece_o;      // [2 grid][heads][d]
   float *piece_ml;     // [2 grid][heads][2]
   int4 *piece_of;      // [grid]: row, unit, pieces of the unit that begins in the CTA's slot 1 (0: none)
 };
 
-template <int D>
+template <int D, int Warps>
 struct AttendShared {
   static constexpr int kRowBytes = D * 2;
   static constexpr int kStageBytes = 2 * kAttendKeys * kRowBytes;   // K then V
-  static constexpr int kRingBytes = kAttendWarps * kAttendStages * kStageBytes;
+  static constexpr int kRingBytes = Warps * kAttendStages * kStageBytes;
 };
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -83,37 +88,43 @@ __device__ __forceinline__ int row_length(const AttentionPlan &p, int row) {
   return min(max(p.a.seq_len[row], 0), p.capacity);
 }
 
-// A row without keys still takes one tile: its zeros have to be written.
-__device__ __forceinline__ int row_tiles(int length) {
-  return max(1, (length + kAttendTile - 1) / kAttendTile);
+// A tile is a step of all warps of a CTA.  A row without keys still takes one:
+// its zeros have to be written.
+template <int Warps>
+__host__ __device__ __forceinline__ int row_tiles(int length) {
+  constexpr int kTile = Warps * kAttendKeys;
+  return length <= kTile ? 1 : (length + kTile - 1) / kTile;
 }
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kAttendThreads, kAttendCtas) attention_kernel(const AttentionPlan p) {
-  using S = AttendShared<D>;
+template <typename T, int D, int NT, int Warps, bool Whole>
+__global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D, NT)) attention_kernel(const AttentionPlan p) {
+  using S = AttendShared<D, Warps>;
+  constexpr int kAttendThreads = Warps * 32, kAttendTile = Warps * kAttendKeys;
   extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ uint32_t live_mask[kAttendWarps][kAttendStages];
-  __shared__ float merge_ml[kAttendWarps][NT * 8][2];
-  __shared__ int scan[kAttendThreads / 32 + 1];
+  __shared__ uint32_t live_mask[Warps][kAttendStages];
+  __shared__ float merge_ml[Warps][NT * 8][2];
+  __shared__ float merge_f[Warps][NT * 8];
+  __shared__ int scan[Warps];
   __shared__ int found[3];
   constexpr int kChunks = D / 8;   // 16-byte chunks of a row
   const AttentionArgs &a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, q2 = (lane & 3) * 2;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if constexpr (!Whole) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // -- this CTA's share of the tiles (row-major, units of a row, tiles of a unit) --
+  // -- this CTA's share of the work (row-major, units of a row; a unit is its
+  // set-up, then its tiles) --
+  constexpr int kSetup = attend_setup(D);
   int row, off, left;
-  if (p.whole) {
+  if constexpr (Whole) {
     row = blockIdx.x / p.units;
-    const int n = row_tiles(row_length(p, row));
-    off = (blockIdx.x - row * p.units) * n;
-    left = n;
+    left = row_tiles<Warps>(row_length(p, row)) + kSetup;
+    off = (blockIdx.x - row * p.units) * left;
   } else {
     const int per = (a.rows + kAttendThreads - 1) / kAttendThreads;
     const int r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
     int mine = 0;
-    for (int r = r0; r < r1; ++r) mine += row_tiles(row_length(p, r));
+    for (int r = r0; r < r1; ++r) mine += row_tiles<Warps>(row_length(p, r)) + kSetup;
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -124,22 +135,22 @@ __global__ void __launch_bounds__(kAttendThreads, kAttendCtas) attention_kernel(
     if (tid == 0) found[0] = -1;
     __syncthreads();
     int total = 0;
-    for (int w = 0; w < kAttendWarps; ++w) {
+    for (int w = 0; w < Warps; ++w) {
       if (w < warp) incl += scan[w];
       total += scan[w];
     }
     total *= p.units;
-    const int share = max(kAttendMinShare, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+    const int share = max(2 * kSetup, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
     const int64_t begin64 = static_cast<int64_t>(blockIdx.x) * share;
     if (begin64 >= total) {
       if (tid == 0) p.piece_of[blockIdx.x] = make_int4(0, 0, 0, 0);
       return;
     }
     const int begin = static_cast<int>(begin64);
-    int before = incl - mine;   // tiles (of one unit per row) before this thread's rows
+    int before = incl - mine;   // work (of one unit per row) before this thread's rows
     if (before * p.units <= begin && begin < incl * p.units) {
       for (int r = r0; r < r1; ++r) {
-        const int n = row_tiles(row_length(p, r));
+        const int n = row_tiles<Warps>(row_length(p, r)) + kSetup;
         if (begin < (before + n) * p.units) {
           found[0] = r;
           found[1] = begin - before * p.units;
@@ -154,7 +165,7 @@ __global__ void __launch_bounds__(kAttendThreads, kAttendCtas) attention_kernel(
     off = found[1];
     left = found[2];
   }
-  const int share_tiles = left;   // the full share wherever a unit goes on after this CTA
+  const int share_work = left;   // the full share wherever a unit goes on after this CTA
   int4 tail = make_int4(0, 0, 0, 0);
 
   uint8_t *const my_ring = ring + warp * kAttendStages * S::kStageBytes;
@@ -162,12 +173,21 @@ __global__ void __launch_bounds__(kAttendThreads, kAttendCtas) attention_kernel(
 
   while (left > 0) {
     const int length = row_length(p, row);
-    const int n = row_tiles(length);
-    const int unit = off / n, t0 = off - unit * n;
-    const int count = min(n - t0, left);
+    const int n = row_tiles<Warps>(length), cost = n + kSetup;
+    const int unit = off / cost, at0 = off - unit * cost;
+    const int take = min(cost - at0, left);
+    const int t0 = max(0, at0 - kSetup), count = max(0, at0 + take - kSetup) - t0;
+    off += take;
+    left -= take;
+    const int row_now = row;
+    if (off == cost * p.units) {
+      off = 0;
+      ++row;
+    }
+    if (count == 0) continue;   // only the set-up of a unit that the next CTA takes
     const int kvh = unit / p.chunks, head0 = kvh * p.groups + (unit - kvh * p.chunks) * p.chunk;
     const int heads = min(p.chunk, (kvh + 1) * p.groups - head0);
-    const int32_t *table = a.block_table + row * a.table_stride;
+    const int32_t *table = a.block_table + row_now * a.table_stride;
     const T *kbase = static_cast<const T *>(a.key_cache) + kvh * D;
     const T *vbase = static_cast<const T *>(a.value_cache) + kvh * D;
 
@@ -176,7 +196,7 @@ __global__ void __launch_bounds__(kAttendThreads, kAttendCtas) attention_kernel(
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int h = nt * 8 + g;
-      const T *qrow = static_cast<const T *>(a.q) + row * a.q_stride + static_cast<int64_t>(head0 + h) * D;
+      const T *qrow = static_cast<const T *>(a.q) + row_now * a.q_stride + static_cast<int64_t>(head0 + h) * D;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         qf[nt][kk][0] = h < heads ? *reinterpret_cast<const uint32_t *>(qrow + kk * 16 + q2) : 0u;
@@ -184,17 +204,23 @@ __global__ void __launch_bounds__(kAttendThreads, kAttendCtas) attention_kernel(
       }
     }
 
+    // the block of this lane's key of step i (-1: none), fetched a step before
+    // its use: the copies of a step do not wait for the table
+    auto block_of = [&](int i) {
+      const int t = (t0 + i) * kAttendTile + warp * kAttendKeys + lane;
+      if (i >= count || lane >= kAttendKeys || t >= length) return -1;
+      return table[p.block_shift >= 0 ? t >> p.block_shift : t / a.block_size];
+    };
+    int next_block = block_of(0);
     auto load = [&](int i, int stage) {
-      const int base = (t0 + i) * kAttendTile + warp * kAttendKeys;
+      const int id = next_block;
+      next_block = block_of(i + 1);
+      const int t = (t0 + i) * kAttendTile + warp * kAttendKeys + lane;
+      const bool live = id >= 0 && id < a.num_blocks;
       int64_t at = 0;
-      bool live = false;
-      if (i < count && lane < kAttendKeys && base + lane < length) {
-        const int t = base + lane;
-        const int blk = p.block_shift >= 0 ? t >> p.block_shift : t / a.block_size;
-        const int in = t - blk * a.block_size;
-        const int id = table[blk];
-        live = id >= 0 && id < a.num_blocks;
-        if (live) at = id * a.block_stride + static_cast<int64_t>(in) * a.nkv * D;
+      if (live) {
+        const int in = p.block_shift >= 0 ? t & (a.block_size - 1) : t % a.block_size;
+        at = id * a.block_stride + static_cast<int64_t>(in) * a.nkv * D;
       }
       const uint32_t mask = __ballot_sync(0xffffffffu, live);
       if (lane == 0) live_mask[warp][stage] = mask;
@@ -233,17 +259,23 @@ __global__ void __launch_bounds__(kAttendThreads, kAttendCtas) attention_kernel(
       load(i + kAttendStages - 1, fill);   // the stage every lane left before the barrier above
       if (mask != 0) {
         const uint32_t kaddr = ring_addr + stage * S::kStageBytes, vaddr = kaddr + kAttendKeys * S::kRowBytes;
-        float s[NT][4];
+        float s[NT][4], s2[NT][4];   // two chains: a product waits for the one before the last
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[nt][j] = s2[nt][j] = 0.f;
         const int krow = lane & 15;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           uint32_t ka[4];
           ldmatrix_x4(ka, kaddr + krow * S::kRowBytes + (((2 * kk + (lane >> 4)) ^ (krow & 7)) << 4));
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) Element<T>::mma(s[nt], ka, qf[nt][kk][0], qf[nt][kk][1]);
+          for (int nt = 0; nt < NT; ++nt) Element<T>::mma(kk & 1 ? s2[nt] : s[nt], ka, qf[nt][kk][0], qf[nt][kk][1]);
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[nt][j] += s2[nt][j];
         const bool live0 = (mask >> g) & 1, live1 = (mask >> (g + 8)) & 1;
         uint32_t pb[NT][2];
 #pragma unroll
@@ -304,6 +336,29 @@ __global__ void __launch_bounds__(kAttendThreads, kAttendCtas) attention_kernel(
       }
     }
     __syncthreads();   // every warp is done with its ring
+    const bool whole = t0 == 0 && count == n;
+    const int64_t piece = 2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0);
+    if (tid < heads) {   // the head's maximum and sum, each warp's factor, lse
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < Warps; ++w) top = fmaxf(top, merge_ml[w][tid][0]);
+      const float base = top == -INFINITY ? 0.f : top;
+      float f[Warps];
+#pragma unroll
+      for (int w = 0; w < Warps; ++w) {
+        f[w] = exp2f(merge_ml[w][tid][0] - base);
+        sum = fmaf(merge_ml[w][tid][1], f[w], sum);
+      }
+      // a whole unit is divided here; no key with a weight gives zeros and log 0
+      const float scale = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int w = 0; w < Warps; ++w) merge_f[w][tid] = f[w] * scale;
+      if (!whole) {
+        *reinterpret_cast<float2 *>(p.piece_ml + (piece * (NT * 8) + tid) * 2) = make_float2(top, sum);
+      } else if (a.lse != nullptr) {
+        a.lse[static_cast<int64_t>(row_now) * a.nq + head0 + tid] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+      }
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float *const h0 = merge + (warp * NT * 8 + nt * 8 + q2) * kStride + g;
@@ -316,51 +371,39 @@ __global__ void __launch_bounds__(kAttendThreads, kAttendCtas) attention_kernel(
       }
     }
     __syncthreads();
-    const bool whole = t0 == 0 && count == n;
-    const int64_t piece = 2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0);
-    for (int i = tid; i < heads * D; i += kAttendThreads) {
-      const int h = i / D, c = i % D;
-      float top = -INFINITY;
+    for (int i = tid; i < heads * (D / 4); i += kAttendThreads) {   // four dimensions a thread
+      const int h = i / (D / 4), c = i % (D / 4) * 4;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kAttendWarps; ++w) top = fmaxf(top, merge_ml[w][h][0]);
-      const float base = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, o = 0.f;
-#pragma unroll
-      for (int w = 0; w < kAttendWarps; ++w) {
-        const float f = exp2f(merge_ml[w][h][0] - base);
-        sum = fmaf(merge_ml[w][h][1], f, sum);
-        o = fmaf(merge[(w * NT * 8 + h) * kStride + c], f, o);
+      for (int w = 0; w < Warps; ++w) {
+        const float f = merge_f[w][h];
+        const float4 v = *reinterpret_cast<const float4 *>(merge + (w * NT * 8 + h) * kStride + c);
+        o.x = fmaf(v.x, f, o.x);
+        o.y = fmaf(v.y, f, o.y);
+        o.z = fmaf(v.z, f, o.z);
+        o.w = fmaf(v.w, f, o.w);
       }
       if (whole) {
-        // no key with a weight: zeros and log 0
-        static_cast<T *>(a.out)[row * a.out_stride + static_cast<int64_t>(head0) * D + i] =
-            Element<T>::round(sum == 0.f ? 0.f : o / sum);
-        if (c == 0 && a.lse != nullptr)
-          a.lse[static_cast<int64_t>(row) * a.nq + head0 + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+        *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + row_now * a.out_stride + static_cast<int64_t>(head0 + h) * D + c) =
+            make_uint2(Element<T>::pack(o.x, o.y), Element<T>::pack(o.z, o.w));
       } else {
-        p.piece_o[piece * (NT * 8 * D) + i] = o;
-        if (c == 0) {
-          p.piece_ml[(piece * (NT * 8) + h) * 2] = top;
-          p.piece_ml[(piece * (NT * 8) + h) * 2 + 1] = sum;
-        }
+        *reinterpret_cast<float4 *>(p.piece_o + piece * (NT * 8 * D) + h * D + c) = o;
       }
     }
     __syncthreads();   // the ring is free for the next segment
-    if (!whole && t0 == 0) tail = make_int4(row, unit, 1 + (n - count + share_tiles - 1) / share_tiles, 0);
-    off += count;
-    left -= count;
-    if (off == n * p.units) {
-      off = 0;
-      ++row;
-    }
+    if (!whole && t0 == 0) tail = make_int4(row_now, unit, 1 + (n - count + share_work - 1) / share_work, 0);
   }
-  if (!p.whole && tid == 0) p.piece_of[blockIdx.x] = tail;
+  if (!Whole && tid == 0) p.piece_of[blockIdx.x] = tail;
 }
 
 // Joins the pieces of the unit that begins in CTA blockIdx.x of the attention
-// and goes on after it; one CTA per (attention CTA, head of the unit).
+// and goes on after it.  D / 4 lanes take a head's row of a piece, four
+// dimensions each; the lanes' groups share the heads and their pieces.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttentionPlan p) {
+__global__ void __launch_bounds__(kJoinThreads, 1) attention_join_kernel(const AttentionPlan p) {
+  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
+  __shared__ __align__(16) float red[kGroups][D];
+  __shared__ float red_ml[kGroups][2];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 of = p.piece_of[blockIdx.x];
   const int pieces = of.z;
@@ -369,51 +412,69 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const Atte
   const int row = of.x, kvh = of.y / p.chunks;
   const int head0 = kvh * p.groups + (of.y - kvh * p.chunks) * p.chunk;
   const int heads = min(p.chunk, (kvh + 1) * p.groups - head0);
-  const int h = blockIdx.y;
-  if (h >= heads) return;
-  constexpr int kLanes = D / 4;                       // 4 dimensions a thread
-  constexpr int kParts = kJoinThreads / kLanes;       // pieces taken in turn
-  __shared__ __align__(16) float red[kParts][D];
-  __shared__ float red_ml[kParts][2];
-  const int c = threadIdx.x % kLanes, part = threadIdx.x / kLanes;
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = part; i < pieces; i += kParts) {
-    // the first piece lies in slot 1 of its CTA, the others in slot 0 of the CTAs after it
-    const int64_t piece = i == 0 ? 2 * static_cast<int64_t>(blockIdx.x) + 1 : 2 * (static_cast<int64_t>(blockIdx.x) + i);
-    const float2 ml = *reinterpret_cast<const float2 *>(p.piece_ml + (piece * (NT * 8) + h) * 2);
-    const float4 v = *reinterpret_cast<const float4 *>(p.piece_o + piece * (NT * 8 * D) + h * D + c * 4);
-    const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.f : top;
-    const float fa = exp2f(m - base), fb = exp2f(ml.x - base);
-    o.x = o.x * fa + v.x * fb;
-    o.y = o.y * fa + v.y * fb;
-    o.z = o.z * fa + v.z * fb;
-    o.w = o.w * fa + v.w * fb;
-    l = l * fa + ml.y * fb;
-    m = top;
-  }
-  *reinterpret_cast<float4 *>(&red[part][c * 4]) = o;
-  if (c == 0) {
-    red_ml[part][0] = m;
-    red_ml[part][1] = l;
+  const int parts = min(kGroups / heads, pieces);   // groups that share a head
+  const int c = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int h = group % heads, part = group / heads;
+  if (part < parts) {
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = part; i0 < pieces; i0 += parts * kJoinBatch) {
+      float2 ml[kJoinBatch];
+      float4 v[kJoinBatch];
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k) {
+        const int i = i0 + k * parts;
+        ml[k] = make_float2(-INFINITY, 0.f);
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < pieces) {
+          // the first piece lies in slot 1 of its CTA, the others in slot 0 of the CTAs after it
+          const int64_t piece = i == 0 ? 2 * static_cast<int64_t>(blockIdx.x) + 1 : 2 * (static_cast<int64_t>(blockIdx.x) + i);
+          ml[k] = *reinterpret_cast<const float2 *>(p.piece_ml + (piece * (NT * 8) + h) * 2);
+          v[k] = *reinterpret_cast<const float4 *>(p.piece_o + piece * (NT * 8 * D) + h * D + c * 4);
+        }
+      }
+      float top = m;
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k) top = fmaxf(top, ml[k].x);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float fa = exp2f(m - base);
+      o.x *= fa;
+      o.y *= fa;
+      o.z *= fa;
+      o.w *= fa;
+      l *= fa;
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k) {
+        const float f = exp2f(ml[k].x - base);
+        o.x = fmaf(v[k].x, f, o.x);
+        o.y = fmaf(v[k].y, f, o.y);
+        o.z = fmaf(v[k].z, f, o.z);
+        o.w = fmaf(v[k].w, f, o.w);
+        l = fmaf(ml[k].y, f, l);
+      }
+      m = top;
+    }
+    *reinterpret_cast<float4 *>(&red[group][c * 4]) = o;
+    if (c == 0) {
+      red_ml[group][0] = m;
+      red_ml[group][1] = l;
+    }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < D; i += kJoinThreads) {
+  for (int i = threadIdx.x; i < heads * D; i += kJoinThreads) {
+    const int head = i / D, d = i % D;
     float top = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kParts; ++k) top = fmaxf(top, red_ml[k][0]);
+    for (int k = 0; k < parts; ++k) top = fmaxf(top, red_ml[k * heads + head][0]);
     const float base = top == -INFINITY ? 0.f : top;
     float sum = 0.f, v = 0.f;
-#pragma unroll
-    for (int k = 0; k < kParts; ++k) {
-      const float f = exp2f(red_ml[k][0] - base);
-      sum = fmaf(red_ml[k][1], f, sum);
-      v = fmaf(red[k][i], f, v);
+    for (int k = 0; k < parts; ++k) {
+      const float f = exp2f(red_ml[k * heads + head][0] - base);
+      sum = fmaf(red_ml[k * heads + head][1], f, sum);
+      v = fmaf(red[k * heads + head][d], f, v);
     }
-    static_cast<T *>(a.out)[row * a.out_stride + static_cast<int64_t>(head0 + h) * D + i] =
-        Element<T>::round(sum == 0.f ? 0.f : v / sum);
-    if (i == 0 && a.lse != nullptr)
-      a.lse[static_cast<int64_t>(row) * a.nq + head0 + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+    static_cast<T *>(a.out)[row * a.out_stride + static_cast<int64_t>(head0) * D + i] = Element<T>::round(sum == 0.f ? 0.f : v / sum);
+    if (d == 0 && a.lse != nullptr)
+      a.lse[static_cast<int64_t>(row) * a.nq + head0 + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
   }
 }
 

@@ -68,11 +68,27 @@ cudaError_t allow_shared(Kernel kernel, size_t bytes, int device, std::atomic<ui
   return err;
 }
 
+// A kernel that joins what the one before it in the stream leaves: it may start
+// while that one drains and waits for it inside (griddepcontrol.wait).
+template <typename... Params, typename... Actual>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, const Actual &...args) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // ---- rotate_store --------------------------------------------------------------
 
 template <typename T, int D>
 cudaError_t rotate_typed(const RotateArgs &a, int device, cudaStream_t stream) {
-  constexpr int kHeads = 256 / D;   // heads a warp moves per round
+  constexpr int kHeads = 512 / D;   // heads a warp moves per round
   const int all = (a.nq + 2 * a.nkv + kHeads - 1) / kHeads;
   // as many rounds per warp as still leave 16 warps per SM: few tokens spread
   // their heads over the GPU, many keep their table row in registers
@@ -95,15 +111,16 @@ struct AttentionShape {
   int grid;   // CTAs of the split form
 };
 
-AttentionShape attention_shape(int32_t rows, int32_t nq, int32_t nkv, int64_t capacity, int device) {
+AttentionShape attention_shape(int32_t rows, int32_t nq, int32_t nkv, int32_t d, int64_t capacity, int device) {
   AttentionShape s;
   s.groups = nq / nkv;
   s.chunks = (s.groups + 15) / 16;
   s.chunk = (s.groups + s.chunks - 1) / s.chunks;
   s.units = nkv * s.chunks;
-  s.whole = capacity <= 8 * kAttendTile;
-  s.grid = sm_count(device) * kAttendCtas;
-  (void)rows;
+  // few short rows: one CTA per unit and no second kernel
+  const int sms = sm_count(device);
+  s.whole = capacity <= 4 * kAttendWholeWarps * kAttendKeys && static_cast<int64_t>(rows) * s.units <= sms;
+  s.grid = sms * attend_ctas(d, s.chunk <= 8 ? 1 : 2);
   return s;
 }
 
@@ -129,34 +146,30 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
   for (int b = 0; b < 31; ++b)
     if (a.block_size == 1 << b) p.block_shift = b;
   p.capacity = a.table_width * a.block_size;
-  p.whole = s.whole ? 1 : 0;
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  if (!s.whole) {
-    size_t ml = 0, of = 0;
-    pieces_bytes(s.grid, NT * 8, D, &ml, &of);
-    uint8_t *w = static_cast<uint8_t *>(a.workspace);
-    p.piece_o = reinterpret_cast<float *>(w);
-    p.piece_ml = reinterpret_cast<float *>(w + ml);
-    p.piece_of = reinterpret_cast<int4 *>(w + of);
+  static std::atomic<uint64_t> done{0}, done_whole{0};
+  if (s.whole) {
+    constexpr size_t smem = AttendShared<D, kAttendWholeWarps>::kRingBytes;
+    auto *kernel = attention_kernel<T, D, NT, kAttendWholeWarps, true>;
+    const cudaError_t err = allow_shared(kernel, smem, device, done_whole);
+    if (err != cudaSuccess) return err;
+    kernel<<<static_cast<unsigned>(a.rows) * s.units, kAttendWholeWarps * 32, smem, stream>>>(p);
+    return cudaGetLastError();
   }
-  static std::atomic<uint64_t> done{0};
-  constexpr size_t smem = AttendShared<D>::kRingBytes;
-  cudaError_t err = allow_shared(attention_kernel<T, D, NT>, smem, device, done);
+  size_t ml = 0, of = 0;
+  pieces_bytes(s.grid, NT * 8, D, &ml, &of);
+  uint8_t *w = static_cast<uint8_t *>(a.workspace);
+  p.piece_o = reinterpret_cast<float *>(w);
+  p.piece_ml = reinterpret_cast<float *>(w + ml);
+  p.piece_of = reinterpret_cast<int4 *>(w + of);
+  constexpr size_t smem = AttendShared<D, kAttendWarps>::kRingBytes;
+  auto *kernel = attention_kernel<T, D, NT, kAttendWarps, false>;
+  cudaError_t err = allow_shared(kernel, smem, device, done);
   if (err != cudaSuccess) return err;
-  const unsigned grid = s.whole ? static_cast<unsigned>(a.rows) * s.units : static_cast<unsigned>(s.grid);
-  attention_kernel<T, D, NT><<<grid, kAttendThreads, smem, stream>>>(p);
+  kernel<<<s.grid, kAttendWarps * 32, smem, stream>>>(p);
   err = cudaGetLastError();
-  if (err != cudaSuccess || s.whole) return err;
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(s.grid, s.chunk);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attention_join_kernel<T, D, NT>, p);
+  if (err != cudaSuccess) return err;
+  return launch_dependent(attention_join_kernel<T, D, NT>, dim3(s.grid), kJoinThreads, stream, p);
 }
 
 template <typename T>
@@ -170,16 +183,19 @@ cudaError_t attention_of(const AttentionArgs &a, const AttentionShape &s, int de
 
 template <typename T>
 cudaError_t choose_typed(const ChooseArgs &a, int device, cudaStream_t stream) {
-  // CTAs per row: enough for two per SM, each with a slice whose words fit
-  // three CTAs to an SM where possible
-  const int64_t want = 2ll * sm_count(device);
+  const int64_t entries = (a.history != nullptr ? a.history_width : 0) + static_cast<int64_t>(a.bias_token != nullptr ? a.bias_width : 0);
+  // as many CTAs per row as the SMs hold, one each: the call is as long as the
+  // chain of a CTA's steps, which a second one on the SM only stretches
+  const int sms = sm_count(device);
   int ctas = 1;
-  while (ctas < kChooseMaxCluster && (static_cast<int64_t>(a.rows) * ctas < want || choose_slice(a.vocab, ctas) > 18 * 1024) &&
-         choose_slice(a.vocab, ctas) > 1024)
+  while (ctas < kChooseMaxCluster &&
+         (choose_shared(choose_slice(a.vocab, ctas), entries) > 100 * 1024 ||
+          (static_cast<int64_t>(a.rows) * ctas * 2 <= sms && choose_slice(a.vocab, ctas) > 4096)))
     ctas *= 2;
-  const size_t smem = static_cast<size_t>(choose_slice(a.vocab, ctas)) * 4;
+  const int32_t slice = choose_slice(a.vocab, ctas);
   static std::atomic<uint64_t> done{0};
-  cudaError_t err = allow_shared(choose_kernel<T>, 200 * 1024, device, done, true);
+  cudaError_t err = allow_shared(choose_kernel<T>, choose_shared(choose_slice(kChooseMaxVocab, kChooseMaxCluster), kMaxIndex),
+                                 device, done, true);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
@@ -189,11 +205,11 @@ cudaError_t choose_typed(const ChooseArgs &a, int device, cudaStream_t stream) {
   attr.val.clusterDim.z = 1;
   cfg.gridDim = dim3(ctas, a.rows);
   cfg.blockDim = dim3(kChooseThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = choose_shared(slice, entries);
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, choose_kernel<T>, a);
+  return cudaLaunchKernelEx(&cfg, choose_kernel<T>, a, slice);
 }
 
 // ---- errors --------------------------------------------------------------------
@@ -239,7 +255,7 @@ cudaError_t launch_rotate_store(const RotateArgs &a, int device, cudaStream_t st
 }
 
 int64_t attention_workspace(int32_t rows, int32_t nq, int32_t nkv, int32_t d, int64_t capacity, int device) {
-  const AttentionShape s = attention_shape(rows, nq, nkv, capacity, device);
+  const AttentionShape s = attention_shape(rows, nq, nkv, d, capacity, device);
   if (s.whole) return 0;
   return static_cast<int64_t>(pieces_bytes(s.grid, s.chunk <= 8 ? 8 : 16, d, nullptr, nullptr));
 }
@@ -247,7 +263,7 @@ int64_t attention_workspace(int32_t rows, int32_t nq, int32_t nkv, int32_t d, in
 cudaError_t launch_paged_attention(const AttentionArgs &a, int device, cudaStream_t stream) {
   if (a.rows == 0) return cudaSuccess;
   const AttentionShape s =
-      attention_shape(a.rows, a.nq, a.nkv, static_cast<int64_t>(a.table_width) * a.block_size, device);
+      attention_shape(a.rows, a.nq, a.nkv, a.d, static_cast<int64_t>(a.table_width) * a.block_size, device);
   return a.dtype == kBf16 ? attention_of<__nv_bfloat16>(a, s, device, stream) : attention_of<__half>(a, s, device, stream);
 }
 
@@ -321,10 +337,11 @@ static int32_t check_attention_sizes(const char *op, int32_t rows, int32_t num_h
   if (rows < 0 || num_kv_heads < 1 || num_heads < 1 || num_heads % num_kv_heads != 0 || num_heads > 1024)
     return refuse("%s: %d rows of %d query heads over %d KV heads (a multiple, at most 1024)", op, rows, num_heads, num_kv_heads);
   if (head_dim != 64 && head_dim != 128) return refuse("%s: head size %d (64 or 128)", op, head_dim);
-  if (capacity < 0 || capacity > kMaxIndex - kAttendTile) return refuse("%s: a capacity of %lld positions (below 2^31)", op, static_cast<long long>(capacity));
+  constexpr int kTile = kAttendWarps * kAttendKeys;
+  if (capacity < 0 || capacity > kMaxIndex - kTile) return refuse("%s: a capacity of %lld positions (below 2^31)", op, static_cast<long long>(capacity));
   const int64_t units = static_cast<int64_t>(num_kv_heads) * ((num_heads / num_kv_heads + 15) / 16);
-  if (rows * units * std::max<int64_t>(1, (capacity + kAttendTile - 1) / kAttendTile) > kMaxIndex)
-    return refuse("%s: rows x KV heads x capacity / %d passes 2^31", op, kAttendTile);
+  if (rows * units * (std::max<int64_t>(1, (capacity + kTile - 1) / kTile) + attend_setup(head_dim)) > kMaxIndex)
+    return refuse("%s: rows x KV heads x capacity / %d passes 2^31", op, kTile);
   return 0;
 }
 
@@ -400,8 +417,8 @@ int32_t cruise_decoder_choose(const void *logits, int64_t logits_stride, int32_t
                               const uint32_t *allowed, int64_t allowed_stride, float *processed,
                               int64_t processed_stride, int64_t *token, int32_t append, int32_t device, void *stream) {
   const char *const op = "cruise_decoder_choose";
-  if (rows < 0 || rows > 65535 || vocab < 1 || vocab > 800000)
-    return refuse("%s: %d rows of %d logits (at most 65535 rows of 1 to 800000)", op, rows, vocab);
+  if (rows < 0 || rows > 65535 || vocab < 1 || vocab > kChooseMaxVocab)
+    return refuse("%s: %d rows of %d logits (at most 65535 rows of 1 to %d)", op, rows, vocab, kChooseMaxVocab);
   if (dtype < kBf16 || dtype > kFp32) return refuse("%s: dtype %d (0 bf16, 1 fp16 or 2 fp32)", op, dtype);
   if (logits_stride < vocab || (processed != nullptr && processed_stride < vocab) ||
       (allowed != nullptr && allowed_stride < (vocab + 31) / 32))

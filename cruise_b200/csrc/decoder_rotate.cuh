@@ -14,102 +14,177 @@
 namespace cruise {
 namespace ops {
 
-constexpr int kRotateThreads = 256;
+constexpr int kRotateThreads = 128;
+constexpr int kRotateBatch = 3;
 
-// 16 bytes (8 elements) per lane: D / 8 lanes share a head, so a warp moves
-// 32 * 8 / D heads of one token per round and takes `rounds` rounds; the
-// token's table row stays in registers over them.
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(*reinterpret_cast<uint64_t *>(&r))
+      : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*reinterpret_cast<uint64_t *>(&r))
+      : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)), "l"(*reinterpret_cast<uint64_t *>(&c)));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack2(const uint4 &u, float2 (&v)[4]) {
+  v[0] = Element<T>::unpack(u.x);
+  v[1] = Element<T>::unpack(u.y);
+  v[2] = Element<T>::unpack(u.z);
+  v[3] = Element<T>::unpack(u.w);
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack2(const float2 (&v)[4]) {
+  return make_uint4(Element<T>::pack(v[0].x, v[0].y), Element<T>::pack(v[1].x, v[1].y), Element<T>::pack(v[2].x, v[2].y),
+                    Element<T>::pack(v[3].x, v[3].y));
+}
+
+// Eight table entries.
+__device__ __forceinline__ void table8(const void *table, int32_t type, int64_t at, float2 (&v)[4]) {
+  if (type == kFp32) {
+    const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(table) + at);
+    const float4 a = p[0], b = p[1];
+    v[0] = make_float2(a.x, a.y);
+    v[1] = make_float2(a.z, a.w);
+    v[2] = make_float2(b.x, b.y);
+    v[3] = make_float2(b.z, b.w);
+  } else {
+    unpack2<__nv_bfloat16>(*reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(table) + at), v);
+  }
+}
+
+// A lane holds two 16-byte chunks of a head: a chunk of the rotated part's
+// first half and its partner half a rotation further (or two neighbours behind
+// the rotated part), so the rotation needs no exchange between lanes.  D / 16
+// lanes share a head, a warp moves 512 / D heads of one token per round and
+// takes `rounds` rounds.  Norm weights and table entries become one factor per
+// element, z_lo = inv (x_lo c_lo + x_hi s_lo), kept in registers over the
+// token's heads.  kRotateBatch rounds of loads are in flight before their first use.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRotateThreads) rotate_store_kernel(const RotateArgs a, int rounds, int warps_per_token) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 16;
   constexpr int kHeads = 32 / kLanes;
   const int64_t warp = (static_cast<int64_t>(blockIdx.x) * kRotateThreads + threadIdx.x) >> 5;
   const int64_t t = warp / warps_per_token;
   if (t >= a.tokens) return;   // uniform over the warp
-  const int first = static_cast<int>(warp - t * warps_per_token) * rounds;
+  const int first = static_cast<int>(warp - t * warps_per_token) * rounds * kHeads;
   const int lane = threadIdx.x & 31;
-  const int chunk = lane % kLanes, sub = lane / kLanes;
+  const int j = lane % kLanes, sub = lane / kLanes;
+  const int half = a.rotary / 16;   // chunks in half the rotated part
+  const bool turns = j < half;
+  const int lo = (turns ? j : 2 * j) * 8, hi = lo + (turns ? half : 1) * 8;   // this lane's elements of a head
+  const int last = min(a.nq + 2 * a.nkv, first + rounds * kHeads);
+  const T *src = static_cast<const T *>(a.qkv) + t * a.qkv_stride;
+  uint4 raw[kRotateBatch][2];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int k = 0; k < kRotateBatch; ++k) {
+      const int head = base + k * kHeads + sub;
+      raw[k][0] = raw[k][1] = make_uint4(0, 0, 0, 0);
+      if (head < last) {
+        raw[k][0] = *reinterpret_cast<const uint4 *>(src + head * D + lo);
+        raw[k][1] = *reinterpret_cast<const uint4 *>(src + head * D + hi);
+      }
+    }
+  };
+  load(first);
   const int64_t pos = a.position[t];
   const int32_t slot = a.slot[t];
   const bool known = pos >= 0 && pos < a.rope_rows;
   const bool stored = known && slot >= 0 && slot < a.num_blocks * a.block_size;
-  const int half = a.rotary / 16;   // chunks in half the rotated part
-  const bool turns = chunk < 2 * half;
-  const int partner = (lane & ~(kLanes - 1)) | (turns ? (chunk < half ? chunk + half : chunk - half) : chunk);
-  float cs[8], sn[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) cs[i] = 1.f, sn[i] = 0.f;
-  if (known && turns) {
-    const int64_t at = pos * a.rotary + chunk * 8;
-    if (a.rope_dtype == kFp32) {
-      const float4 *c = reinterpret_cast<const float4 *>(static_cast<const float *>(a.rope_cos) + at);
-      const float4 *s = reinterpret_cast<const float4 *>(static_cast<const float *>(a.rope_sin) + at);
-      const float4 c0 = c[0], c1 = c[1], s0 = s[0], s1 = s[1];
-      cs[0] = c0.x; cs[1] = c0.y; cs[2] = c0.z; cs[3] = c0.w; cs[4] = c1.x; cs[5] = c1.y; cs[6] = c1.z; cs[7] = c1.w;
-      sn[0] = s0.x; sn[1] = s0.y; sn[2] = s0.z; sn[3] = s0.w; sn[4] = s1.x; sn[5] = s1.y; sn[6] = s1.z; sn[7] = s1.w;
-    } else {
-      unpack8<__nv_bfloat16>(*reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.rope_cos) + at), cs);
-      unpack8<__nv_bfloat16>(*reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.rope_sin) + at), sn);
-    }
-    if (chunk < half) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sn[i] = -sn[i];
-    }
-  }
   const bool norm = a.q_norm != nullptr;
-  uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;
-  if (norm) {
-    wq = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q_norm) + chunk * 8);
-    wk = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.k_norm) + chunk * 8);
-  }
-  const T *src = static_cast<const T *>(a.qkv) + t * a.qkv_stride + chunk * 8;
-  T *q_dst = static_cast<T *>(a.q_out) + t * a.q_stride + chunk * 8;
-  const int64_t cell = stored ? (slot / a.block_size) * a.block_stride +
-                                    static_cast<int64_t>(slot % a.block_size) * a.nkv * D + chunk * 8
-                              : 0;
+  T *q_dst = static_cast<T *>(a.q_out) + t * a.q_stride;
+  const int64_t cell = stored ? (slot / a.block_size) * a.block_stride + static_cast<int64_t>(slot % a.block_size) * a.nkv * D : 0;
   T *k_dst = static_cast<T *>(a.key_cache) + cell;
   T *v_dst = static_cast<T *>(a.value_cache) + cell;
-  const int heads = a.nq + 2 * a.nkv;
-  const int last = min(heads, (first + rounds) * kHeads);
-#pragma unroll 4
-  for (int base = first * kHeads; base < last; base += kHeads) {
-    const int head = base + sub;
-    const bool live = head < heads;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (live) raw = *reinterpret_cast<const uint4 *>(src + static_cast<int64_t>(head) * D);
-    if (base >= a.nq + a.nkv) {   // v heads only: copied as they are
-      if (live && stored)
-        *reinterpret_cast<uint4 *>(v_dst + static_cast<int64_t>(head - a.nq - a.nkv) * D) = raw;
-      continue;
-    }
-    float y[8];
-    unpack8<T>(raw, y);
-    if (norm) {
-      float ss = 0.f;
+  // z_lo = x_lo c_lo + x_hi s_lo, z_hi = x_hi c_hi + x_lo s_hi (times the head's inverse norm)
+  float2 c_lo[4], c_hi[4], s_lo[4], s_hi[4];
+  int built = -1;   // whose factors the lane holds: 0 query heads, 1 key heads
+  for (int base = first; base < last; base += kRotateBatch * kHeads) {
+    if (base > first) load(base);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
+    for (int k = 0; k < kRotateBatch; ++k) {
+      const int begin = base + k * kHeads, head = begin + sub;
+      if (begin >= last) break;   // uniform over the warp
+      if (begin < a.nq + a.nkv) {
+        const int kind = norm && head >= a.nq ? 1 : 0;
+        if (built != kind) {
 #pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float inv = rsqrtf(ss * (1.f / D) + a.eps);
-      float w[8];
-      unpack8<T>(head < a.nq ? wq : wk, w);
+          for (int i = 0; i < 4; ++i) {
+            c_lo[i] = c_hi[i] = make_float2(1.f, 1.f);
+            s_lo[i] = s_hi[i] = make_float2(0.f, 0.f);
+          }
+          if (known && turns) {
+            table8(a.rope_cos, a.rope_dtype, pos * a.rotary + lo, c_lo);
+            table8(a.rope_cos, a.rope_dtype, pos * a.rotary + hi, c_hi);
+            table8(a.rope_sin, a.rope_dtype, pos * a.rotary + lo, s_lo);
+            table8(a.rope_sin, a.rope_dtype, pos * a.rotary + hi, s_hi);
+          }
+          if (norm) {
+            const T *weight = static_cast<const T *>(kind == 0 ? a.q_norm : a.k_norm);
+            float2 w_lo[4], w_hi[4];
+            unpack2<T>(*reinterpret_cast<const uint4 *>(weight + lo), w_lo);
+            unpack2<T>(*reinterpret_cast<const uint4 *>(weight + hi), w_hi);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = y[i] * inv * w[i];
-    }
-    float z[8];
+            for (int i = 0; i < 4; ++i) {
+              c_lo[i] = mul2(c_lo[i], w_lo[i]);
+              c_hi[i] = mul2(c_hi[i], w_hi[i]);
+              s_lo[i] = mul2(s_lo[i], w_hi[i]);
+              s_hi[i] = mul2(s_hi[i], w_lo[i]);
+            }
+          }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float other = __shfl_sync(0xffffffffu, y[i], partner);
-      z[i] = turns ? fmaf(other, sn[i], y[i] * cs[i]) : y[i];
-    }
-    if (!live) continue;
-    if (head < a.nq) {
-      *reinterpret_cast<uint4 *>(q_dst + static_cast<int64_t>(head) * D) = known ? pack8<T>(z) : make_uint4(0, 0, 0, 0);
-    } else if (stored) {
-      if (head < a.nq + a.nkv)
-        *reinterpret_cast<uint4 *>(k_dst + static_cast<int64_t>(head - a.nq) * D) = pack8<T>(z);
-      else
-        *reinterpret_cast<uint4 *>(v_dst + static_cast<int64_t>(head - a.nq - a.nkv) * D) = raw;
+          for (int i = 0; i < 4; ++i) s_lo[i] = make_float2(-s_lo[i].x, -s_lo[i].y);
+          built = kind;
+        }
+        float2 x_lo[4], x_hi[4];
+        unpack2<T>(raw[k][0], x_lo);
+        unpack2<T>(raw[k][1], x_hi);
+        float inv = 1.f;
+        if (norm) {
+          float2 ss = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            ss = fma2(x_lo[i], x_lo[i], ss);
+            ss = fma2(x_hi[i], x_hi[i], ss);
+          }
+          float sum = ss.x + ss.y;
+#pragma unroll
+          for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          inv = rsqrtf(sum * (1.f / D) + a.eps);
+        }
+        const float2 inv2 = make_float2(inv, inv);
+        float2 z_lo[4], z_hi[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          z_lo[i] = mul2(x_lo[i], c_lo[i]);
+          z_hi[i] = mul2(x_hi[i], c_hi[i]);
+          if (turns) {
+            z_lo[i] = fma2(x_hi[i], s_lo[i], z_lo[i]);
+            z_hi[i] = fma2(x_lo[i], s_hi[i], z_hi[i]);
+          }
+          z_lo[i] = mul2(z_lo[i], inv2);
+          z_hi[i] = mul2(z_hi[i], inv2);
+        }
+        if (head < a.nq + a.nkv) {
+          raw[k][0] = pack2<T>(z_lo);
+          raw[k][1] = pack2<T>(z_hi);
+        }
+      }
+      if (head >= last) continue;
+      if (head < a.nq && !known) raw[k][0] = raw[k][1] = make_uint4(0, 0, 0, 0);
+      if (head >= a.nq && !stored) continue;
+      T *dst = head < a.nq ? q_dst + head * D : head < a.nq + a.nkv ? k_dst + (head - a.nq) * D : v_dst + (head - a.nq - a.nkv) * D;
+      *reinterpret_cast<uint4 *>(dst + lo) = raw[k][0];
+      *reinterpret_cast<uint4 *>(dst + hi) = raw[k][1];
     }
   }
 }

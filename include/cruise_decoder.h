@@ -93,7 +93,8 @@ int64_t cruise_decoder_attention_workspace(int32_t rows, int32_t num_heads,
  * the token's occurrences after the prompt.  Entries outside the vocabulary do
  * not count.  repetition, frequency, presence: [rows] fp32, NULL for 1, 0, 0.
  * bias_token, bias_value [rows][bias_width] (rows bias_stride apart) with
- * bias_len[r] entries, strictly increasing tokens within a row.  allowed: bit
+ * bias_len[r] entries, increasing tokens within a row (entries of one token add
+ * up).  allowed: bit
  * n % 32 of word n / 32 of a row (rows allowed_stride words apart).  active
  * [rows]: rows with 0 get token -1, nothing else of theirs is written.  Each
  * group may be NULL.
@@ -103,7 +104,7 @@ int64_t cruise_decoder_attention_workspace(int32_t rows, int32_t num_heads,
  * same stride), else must not overlap them.  append: token[r] >= 0 is written to
  * history[r][history_len[r]] where that is inside history_width (history_len
  * itself is the caller's to advance).  4-byte alignment suffices (logits: their
- * own size).  vocab at most 800000. */
+ * own size).  vocab at most 393216. */
 int32_t cruise_decoder_choose(
     const void *logits, int64_t logits_stride, int32_t rows, int32_t vocab,
     int32_t dtype, const int32_t *active, int32_t *history,
