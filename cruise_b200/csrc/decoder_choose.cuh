@@ -11,14 +11,18 @@
 //
 // A cluster of CTAs shares a row, a slice of the vocabulary each; the slices'
 // maxima meet in the first CTA's shared memory, so a call is one launch and
-// keeps no state.  Few tokens of a slice are in the history or the bias list: a
-// bit map in shared memory marks them, their rank in it (a scan of the words'
-// bit counts) is their place in a table of occurrences and a list.  The stream
-// over the slice masks the logits and takes the maximum of the unmarked tokens,
-// a few operations an element; the marked tokens follow, one a thread.
+// keeps no state.  Few tokens of a slice are in the history or the bias list.  Four
+// warps deal with them: a bit map in shared memory marks them, their rank in it
+// is their place in a table of occurrences, and from that come their processed
+// values.  Meanwhile the other warps stream over the slice and know nothing of
+// it: they mask the logits and keep each thread's maximum, a few operations an
+// element.  After the barrier between the two, a thread whose maximum is a marked
+// token has its elements gone over again without them, by a warp together, and
+// the marked tokens' values are written over the stream's.
 #pragma once
 
 #include <climits>
+#include <type_traits>
 
 #include "decoder_common.cuh"
 #include "decoder_ops.h"
@@ -27,12 +31,14 @@ namespace cruise {
 namespace ops {
 
 constexpr int kChooseThreads = 512;
-constexpr int kChooseCtas = 2;           // CTAs per SM
+constexpr int kChooseTableThreads = 128;   // of them, those of the marked tokens
+constexpr int kChooseStreamThreads = kChooseThreads - kChooseTableThreads;
+constexpr int kChooseCtas = 2;             // CTAs per SM
 constexpr int kChooseMaxCluster = 16;
-constexpr int kChooseAhead = 4;          // vectors a thread has in flight
-constexpr int kChooseWindow = kChooseAhead * kChooseThreads;
-constexpr int kChooseBatch = 4;          // history entries a thread has in flight
-constexpr int32_t kChooseMaxVocab = 393216;
+constexpr int kChooseAhead = 4;            // vectors a thread has in flight
+constexpr int kChooseBatch = 8;            // history entries a thread has in flight
+constexpr size_t kChooseShared = 200 * 1024;
+constexpr int32_t kChooseMaxVocab = 1 << 20;
 constexpr uint32_t kInPrompt = 0x80000000u, kHasBias = 0x40000000u, kCount = 0x3fffffffu;
 
 struct ChooseBest {
@@ -76,6 +82,29 @@ __device__ __forceinline__ void store_cluster(void *local, uint32_t rank, uint32
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
+// Tokens of a CTA's slice: a multiple of 32, so that slices share no mask word.
+inline int32_t choose_slice(int32_t vocab, int32_t ctas) { return ((vocab + ctas - 1) / ctas + 31) / 32 * 32; }
+
+// Marked tokens of a slice at most.
+__host__ __device__ inline int32_t choose_listed(int32_t slice, int64_t entries) {
+  return static_cast<int32_t>(entries < slice ? entries : slice);
+}
+
+// Words of a slice's marks, a multiple of 4.
+__host__ __device__ inline int32_t choose_words(int32_t slice) { return (slice / 32 + 3) / 4 * 4; }
+
+// Shared memory of a slice: marks and ranks per word, occurrences and tokens listed.
+inline size_t choose_shared(int32_t slice, int64_t entries) {
+  return static_cast<size_t>(choose_words(slice)) * 8 + static_cast<size_t>(choose_listed(slice, entries)) * 8;
+}
+
+// The larger value; NaN when either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <typename T>
 struct Logit;
 template <>
@@ -100,151 +129,111 @@ struct Logit<__nv_bfloat16> : LogitHalf<__nv_bfloat16> {};
 template <>
 struct Logit<__half> : LogitHalf<__half> {};
 
-// The larger value; NaN when either is.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
-// `count` <= 32 bits from bit n of a bit array.
-__device__ __forceinline__ uint32_t bits_at(const uint32_t *words, int32_t n, int count) {
-  const int32_t w = n >> 5, s = n & 31;
-  uint32_t bits = words[w] >> s;
-  if (s + count > 32) bits |= words[w + 1] << (32 - s);
-  return bits;
-}
-
-// Tokens of a CTA's slice: a multiple of 32, so that slices share no mask word.
-inline int32_t choose_slice(int32_t vocab, int32_t ctas) { return ((vocab + ctas - 1) / ctas + 31) / 32 * 32; }
-
-// Shared memory of a slice with up to `entries` history and bias entries:
-// marks and their ranks per word, occurrences and the list per marked token.
-__host__ __device__ inline int32_t choose_listed(int32_t slice, int64_t entries) {
-  return static_cast<int32_t>(entries < slice ? entries : slice);
-}
-
-inline size_t choose_shared(int32_t slice, int64_t entries) {
-  return static_cast<size_t>(slice) / 32 * 8 + static_cast<size_t>(choose_listed(slice, entries)) * 8;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(const ChooseArgs a, const int32_t slice) {
   extern __shared__ __align__(16) uint32_t shared[];
   __shared__ ChooseBest warp_part[kChooseThreads / 32];
   __shared__ ChooseBest parts[kChooseMaxCluster];
-  __shared__ int32_t scan[kChooseThreads / 32];
+  __shared__ int32_t scan[kChooseTableThreads / 32];
+  __shared__ int32_t shared_listed;   // marked tokens of the slice
+  __shared__ int32_t retakes;         // stream threads whose maximum is one of them
+  __shared__ uint16_t retake_list[kChooseStreamThreads];
   constexpr int kVec = Logit<T>::kVec;
   const int tid = threadIdx.x, row = blockIdx.y, ctas = gridDim.x;
-  const int part = static_cast<int>(cluster_rank());
-  cluster_arrive();   // every CTA of the cluster runs before its shared memory is written
-  const int32_t words = slice / 32;
-  uint32_t *const marks = shared, *const ranks = marks + words, *const counts = ranks + words;
+  const int part = ctas > 1 ? static_cast<int>(cluster_rank()) : 0;
+  if (ctas > 1) cluster_arrive();   // every CTA of the cluster runs before its shared memory is written
   const int32_t v0 = min(part * slice, a.vocab);
   const int32_t width = min(slice, a.vocab - v0);
-  const T *logits = static_cast<const T *>(a.logits) + row * a.logits_stride + v0;
-  const uint32_t *allowed = a.allowed != nullptr ? a.allowed + row * a.allowed_stride + v0 / 32 : nullptr;
+  const T *const logits = static_cast<const T *>(a.logits) + row * a.logits_stride + v0;
+  const uint32_t *const allowed = a.allowed != nullptr ? a.allowed + row * a.allowed_stride + v0 / 32 : nullptr;
+  float *const out = a.processed != nullptr ? a.processed + row * a.processed_stride + v0 : nullptr;
+  const int32_t *const bias_token = a.bias_token != nullptr ? a.bias_token + row * a.bias_stride : nullptr;
   // the row need not begin on a 16-byte boundary: single tokens up to the first one
   const int32_t lead = min(width, static_cast<int32_t>(((16 - (reinterpret_cast<uintptr_t>(logits) & 15)) & 15) / sizeof(T)));
   const int32_t vectors = (width - lead) / kVec;
   const int32_t rest = lead + vectors * kVec;
-  uint4 ahead[kChooseAhead];
-  uint32_t open[kChooseAhead], open_next[kChooseAhead];   // their mask words, as loaded
-  auto fetch = [&](int k, int32_t i) {   // nothing here waits for a load
-    if (i < vectors) {
-      ahead[k] = __ldcs(reinterpret_cast<const uint4 *>(logits + lead) + i);
-      if (allowed != nullptr) {
-        const int32_t n = lead + i * kVec;
-        open[k] = allowed[n >> 5];
-        if ((n & 31) > 32 - kVec) open_next[k] = allowed[(n >> 5) + 1];
-      }
-    }
-  };
-  auto ahead_l2 = [&](int32_t first) {
-    if (first < vectors)
-      prefetch_l2(reinterpret_cast<const uint4 *>(logits + lead) + first, min(kChooseWindow, vectors - first) * 16);
-  };
+  const int32_t steps = (vectors + kChooseStreamThreads - 1) / kChooseStreamThreads;
+  const int32_t last_word = (width - 1) >> 5;
+  const bool split = lead % kVec != 0;   // a vector's mask bits may go on in the next word
+  const uint4 *const stream = reinterpret_cast<const uint4 *>(logits + lead);
   const bool active = a.active == nullptr || a.active[row] != 0;
   ChooseBest best{-INFINITY, INT_MAX, 0};
+  const int32_t words = choose_words(slice);
+  uint32_t *const marks = shared, *const ranks = marks + words, *const counts = ranks + words;
+  uint32_t *const list = counts + choose_listed(slice, static_cast<int64_t>(a.history != nullptr ? a.history_width : 0) +
+                                                           (bias_token != nullptr ? a.bias_width : 0));
+  auto masked = [&](float (&x)[kVec], uint32_t bits) {   // -inf where a bit is 0
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) x[j] = bits & (1u << j) ? x[j] : -INFINITY;
+  };
+  auto open_at = [&](int32_t n) { return allowed == nullptr || ((allowed[n >> 5] >> (n & 31)) & 1u); };
+  float top = -INFINITY;
+  int32_t top_at = -1;
+  if (tid == 0) retakes = 0;
 
-  if (active) {
-#pragma unroll
-    for (int k = 0; k < kChooseAhead; ++k) fetch(k, k * kChooseThreads + tid);
-    // the two windows of the stream after the one in registers, into L2
-    if (tid == 0) {
-      ahead_l2(kChooseWindow);
-      ahead_l2(2 * kChooseWindow);
-    }
-    // the thread's first history and bias entries are fetched with the lengths
-    // that say which of them count
-    const int32_t *history = a.history + (a.history != nullptr ? row * a.history_stride : 0);
-    const int32_t *bias_token = a.bias_token + (a.bias_token != nullptr ? row * a.bias_stride : 0);
-    const float *bias_value = a.bias_value + (a.bias_token != nullptr ? row * a.bias_stride : 0);
-    int32_t kept[kChooseBatch];
-#pragma unroll
-    for (int k = 0; k < kChooseBatch; ++k) {
-      const int32_t i = k * kChooseThreads + tid;
-      kept[k] = a.history != nullptr && i < a.history_width ? history[i] : -1;
-    }
-    const bool has_bias = a.bias_token != nullptr && tid < a.bias_width;
-    int32_t bias_id = has_bias ? bias_token[tid] : -1;
-    const int32_t bias_before = has_bias && tid > 0 ? bias_token[tid - 1] : -1;
-    const int32_t length = a.history != nullptr ? min(max(a.history_len[row], 0), a.history_width) : 0;
-    const int32_t prompt = a.history != nullptr ? min(max(a.prompt_len[row], 0), length) : 0;
-    const float rep = a.repetition != nullptr ? a.repetition[row] : 1.f;
-    const float freq = a.frequency != nullptr ? a.frequency[row] : 0.f;
-    const float pres = a.presence != nullptr ? a.presence[row] : 0.f;
-    const int32_t counted = rep != 1.f || freq != 0.f || pres != 0.f ? length : 0;
-    const int32_t biases = a.bias_token != nullptr ? min(max(a.bias_len[row], 0), a.bias_width) : 0;
-    const int32_t entries = counted + biases;
-    if (tid >= biases) bias_id = -1;
-    uint32_t *const list = counts + choose_listed(slice, static_cast<int64_t>(a.history != nullptr ? a.history_width : 0) +
-                                                             (a.bias_token != nullptr ? a.bias_width : 0));
-    int32_t listed = 0;
-    // this thread's first marked token and bias entry are fetched before the
-    // stream and used after it
-    T bias_x{}, listed_x{};
-    // a vocabulary id as a token of this slice (-1: of another)
-    auto here = [&](int32_t id) {
-      const int64_t n = static_cast<int64_t>(id) - v0;
-      return n >= 0 && n < width ? static_cast<int32_t>(n) : -1;
-    };
-    // f(entry, token) for the entries of this slice: the history's, a batch of
-    // loads in flight, then the bias list's
-    auto each = [&](auto &&f) {
+  if (active && tid < kChooseTableThreads) {
+    // -- the marked tokens; the first history entries are fetched with the lengths
+    // that say which of them count --
+    const int32_t *const history = a.history != nullptr ? a.history + row * a.history_stride : nullptr;
+    const int32_t history_width = history != nullptr ? a.history_width : 0;
+    int32_t first_id[kChooseBatch];
+    auto fetch = [&](int32_t (&id)[kChooseBatch], int32_t i0, int32_t end) {
 #pragma unroll
       for (int k = 0; k < kChooseBatch; ++k) {
-        const int32_t i = k * kChooseThreads + tid, n = here(kept[k]);
-        if (i < counted && n >= 0) f(i, n);
-      }
-      for (int32_t i0 = kChooseBatch * kChooseThreads + tid; i0 < counted; i0 += kChooseBatch * kChooseThreads) {
-        int32_t id[kChooseBatch];
-#pragma unroll
-        for (int k = 0; k < kChooseBatch; ++k) id[k] = i0 + k * kChooseThreads < counted ? history[i0 + k * kChooseThreads] : -1;
-#pragma unroll
-        for (int k = 0; k < kChooseBatch; ++k) {
-          const int32_t n = here(id[k]);
-          if (n >= 0) f(i0 + k * kChooseThreads, n);
-        }
-      }
-      if (here(bias_id) >= 0) f(counted, here(bias_id));
-      for (int32_t i = kChooseThreads + tid; i < biases; i += kChooseThreads) {
-        const int32_t n = here(bias_token[i]);
-        if (n >= 0) f(counted + i, n);
+        const int32_t i = i0 + k * kChooseTableThreads;
+        id[k] = i < end ? history[i] : -1;
       }
     };
-    auto rank = [&](int32_t n) { return ranks[n >> 5] + __popc(marks[n >> 5] & ((1u << (n & 31)) - 1)); };
-    if (entries > 0) {
-      for (int i = tid; i < words; i += kChooseThreads) marks[i] = 0;
-      for (int i = tid; i < min(entries, slice); i += kChooseThreads) counts[i] = 0;
-      __syncthreads();
-      each([&](int32_t, int32_t n) { atomicOr(&marks[n >> 5], 1u << (n & 31)); });
-      __syncthreads();
+    fetch(first_id, tid, history_width);
+    int32_t length = 0, prompt = 0, biases = 0;
+    float rep = 1.f, freq = 0.f, pres = 0.f;
+    if (history != nullptr) {
+      length = a.history_len[row];
+      prompt = a.prompt_len[row];
+    }
+    if (bias_token != nullptr) biases = min(max(a.bias_len[row], 0), a.bias_width);
+    if (a.repetition != nullptr) rep = a.repetition[row];
+    if (a.frequency != nullptr) freq = a.frequency[row];
+    if (a.presence != nullptr) pres = a.presence[row];
+    const int32_t counted = rep != 1.f || freq != 0.f || pres != 0.f ? min(max(length, 0), history_width) : 0;
+    int32_t listed = 0;
+    if (counted + biases > 0) {
+      // a vocabulary id as a token of this slice; others are at least `width`
+      auto here = [&](int32_t id) { return static_cast<uint32_t>(id) - static_cast<uint32_t>(v0); };
+      // f(entry, token) for the slice's entries of the history
+      auto each = [&](auto &&f) {
+        int32_t id[kChooseBatch];
+#pragma unroll
+        for (int k = 0; k < kChooseBatch; ++k) id[k] = first_id[k];
+        for (int32_t i0 = tid; i0 < counted; i0 += kChooseBatch * kChooseTableThreads) {
+          if (i0 != tid) fetch(id, i0, counted);
+#pragma unroll
+          for (int k = 0; k < kChooseBatch; ++k) {
+            const int32_t i = i0 + k * kChooseTableThreads;
+            const uint32_t n = here(id[k]);
+            if (i < counted && n < static_cast<uint32_t>(width)) f(i, n);
+          }
+        }
+      };
+      auto rank = [&](uint32_t n) { return ranks[n >> 5] + __popc(marks[n >> 5] & ((1u << (n & 31)) - 1)); };
+      for (int32_t i = tid; i < words / 4; i += kChooseTableThreads) reinterpret_cast<uint4 *>(marks)[i] = make_uint4(0, 0, 0, 0);
+      const int32_t most = min(counted + biases, width);
+      for (int32_t i = tid; i < most; i += kChooseTableThreads) counts[i] = 0;
+      named_sync(1, kChooseTableThreads);
+      each([&](int32_t, uint32_t n) { atomicOr(&marks[n >> 5], 1u << (n & 31)); });
+      for (int32_t i = tid; i < biases; i += kChooseTableThreads) {
+        const uint32_t n = here(bias_token[i]);
+        if (n < static_cast<uint32_t>(width)) atomicOr(&marks[n >> 5], 1u << (n & 31));
+      }
+      named_sync(1, kChooseTableThreads);
       // ranks: every thread its run of words
-      const int32_t per = (words + kChooseThreads - 1) / kChooseThreads;
+      const int32_t per = (words / 4 + kChooseTableThreads - 1) / kChooseTableThreads * 4;
       const int32_t w0 = min(tid * per, words), w1 = min(w0 + per, words);
       int32_t mine = 0;
-      for (int32_t w = w0; w < w1; ++w) mine += __popc(marks[w]);
+      for (int32_t w = w0; w < w1; w += 4) {
+        const uint4 m = *reinterpret_cast<const uint4 *>(marks + w);
+        mine += __popc(m.x) + __popc(m.y) + __popc(m.z) + __popc(m.w);
+      }
       int32_t incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -252,141 +241,223 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
         if ((tid & 31) >= o) incl += v;
       }
       if ((tid & 31) == 31) scan[tid >> 5] = incl;
-      __syncthreads();
+      named_sync(1, kChooseTableThreads);
 #pragma unroll
-      for (int w = 0; w < kChooseThreads / 32; ++w) {
+      for (int w = 0; w < kChooseTableThreads / 32; ++w) {
         if (w < (tid >> 5)) incl += scan[w];
         listed += scan[w];
       }
-      int32_t at = incl - mine;
-      for (int32_t w = w0; w < w1; ++w) {
-        ranks[w] = at;
-        at += __popc(marks[w]);
+      uint32_t at = incl - mine;
+      for (int32_t w = w0; w < w1; w += 4) {
+        const uint4 m = *reinterpret_cast<const uint4 *>(marks + w);
+        const uint32_t b = at + __popc(m.x), c = b + __popc(m.y), d = c + __popc(m.z);
+        *reinterpret_cast<uint4 *>(ranks + w) = make_uint4(at, b, c, d);
+        at = d + __popc(m.w);
       }
-      __syncthreads();
-      each([&](int32_t i, int32_t n) {
-        const int32_t r = rank(n);
+      named_sync(1, kChooseTableThreads);
+      each([&](int32_t i, uint32_t n) {
+        const uint32_t r = rank(n);
         list[r] = n;   // the token's entries agree
-        if (i >= counted)
-          atomicOr(&counts[r], kHasBias);
-        else if (i < prompt)
+        if (i < prompt)
           atomicOr(&counts[r], kInPrompt);
         else
           atomicAdd(&counts[r], 1u);
       });
-      __syncthreads();
-      if (tid < listed) listed_x = logits[list[tid]];
-      if (here(bias_id) >= 0) bias_x = logits[here(bias_id)];
-    }
-    float *out = a.processed != nullptr ? a.processed + row * a.processed_stride + v0 : nullptr;
-    const bool out16 = (reinterpret_cast<uintptr_t>(out + lead) & 15) == 0;
-
-    auto one = [&](int32_t n) {   // a single token
-      const bool allow = allowed == nullptr || bits_at(allowed, n, 1) & 1u;
-      const bool marked = entries > 0 && (bits_at(marks, n, 1) & 1u);
-      const float x = allow ? Logit<T>::one(logits + n) : -INFINITY;
-      if (out != nullptr) out[n] = x;
-      if (marked) return;
-      if (!(x < INFINITY)) best.bad = 1;   // NaN or +inf
-      if (x > -INFINITY) better(best, x, v0 + n);
-    };
-    if (tid < lead) one(tid);
-    for (int32_t first = 0; first < vectors; first += kChooseWindow) {
-      if (tid == 0) ahead_l2(first + 3 * kChooseWindow);
-#pragma unroll
-      for (int k = 0; k < kChooseAhead; ++k) {
-        const int32_t i = first + k * kChooseThreads + tid;
-        if (i >= vectors) break;
-        const int32_t n = lead + i * kVec;
-        float x[kVec];
-        Logit<T>::unpack(ahead[k], x);
-        if (allowed != nullptr) {
-          const uint32_t bits = __funnelshift_r(open[k], open_next[k], n & 31);
-#pragma unroll
-          for (int j = 0; j < kVec; ++j) x[j] = (bits >> j) & 1u ? x[j] : -INFINITY;
-        }
-        fetch(k, i + kChooseWindow);
-        if (out != nullptr) {
-          if (out16) {
-#pragma unroll
-            for (int j = 0; j < kVec; j += 4)
-              __stcs(reinterpret_cast<float4 *>(out + n + j), make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) out[n + j] = x[j];
-          }
-        }
-        if (entries > 0) {
-          const uint32_t marked = bits_at(marks, n, kVec) & ((1u << kVec) - 1);
-          if (marked != 0) {
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) x[j] = (marked >> j) & 1u ? -INFINITY : x[j];
-          }
-        }
-        float top = x[0];
-#pragma unroll
-        for (int j = 1; j < kVec; ++j) top = max_nan(top, x[j]);
-        if (!(top < INFINITY)) best.bad = 1;
-        if (top > best.value) {   // the thread's tokens come in order: a later equal one loses
-          best.value = top;
-#pragma unroll
-          for (int j = kVec - 1; j >= 0; --j)
-            if (x[j] == top) best.index = v0 + n + j;
+      for (int32_t i = tid; i < biases; i += kChooseTableThreads) {
+        const uint32_t n = here(bias_token[i]);
+        if (n < static_cast<uint32_t>(width)) {
+          const uint32_t r = rank(n);
+          list[r] = n;
+          atomicOr(&counts[r], kHasBias);
         }
       }
-    }
-    if (tid < width - rest) one(rest + tid);
-
-    if (entries > 0) {
-      __syncthreads();
-      // a marked token, its bias added
-      auto rules = [&](int32_t n, uint32_t word, float x) {
-        const uint32_t times = word & kCount;
+      named_sync(1, kChooseTableThreads);
+      // the processed value takes the place of the occurrences
+      auto rules = [&](uint32_t n, uint32_t r, float x) {
+        const uint32_t word = counts[r], times = word & kCount;
         if (word & (kInPrompt | kCount)) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
         if (times != 0) {
           x = __fsub_rn(x, __fmul_rn(freq, static_cast<float>(times)));
           x = __fsub_rn(x, pres);
         }
-        if (allowed != nullptr && (bits_at(allowed, n, 1) & 1u) == 0) x = -INFINITY;
-        if (out != nullptr) out[n] = x;
-        if (!(x < INFINITY)) best.bad = 1;
-        if (x > -INFINITY) better(best, x, v0 + n);
+        if (!open_at(n)) x = -INFINITY;
+        counts[r] = __float_as_uint(x);
+        if (!(x < INFINITY)) best.bad = 1;   // NaN or +inf
+        if (x > -INFINITY) better(best, x, v0 + static_cast<int32_t>(n));
       };
-      for (int32_t i = tid; i < listed; i += kChooseThreads) {
-        const int32_t n = static_cast<int32_t>(list[i]);
-        if ((counts[i] & kHasBias) == 0) rules(n, counts[i], Logit<T>::one(i == tid ? &listed_x : logits + n));
+      // (in place, the stream may have masked a logit already: -inf then, as here)
+      constexpr int kTogether = 4;
+      for (int32_t i0 = tid; i0 < listed; i0 += kTogether * kChooseTableThreads) {
+        T raw[kTogether];
+        uint32_t n[kTogether];
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k) {
+          n[k] = list[min(i0 + k * kChooseTableThreads, listed - 1)];
+          raw[k] = logits[n[k]];
+        }
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k) {
+          const int32_t i = i0 + k * kChooseTableThreads;
+          if (i < listed && (counts[i] & kHasBias) == 0) rules(n[k], i, Logit<T>::one(&raw[k]));
+        }
       }
-      for (int32_t i = tid; i < biases; i += kChooseThreads) {
-        const int32_t id = i == tid ? bias_id : bias_token[i], n = here(id);
-        if (n < 0 || (i > 0 && (i == tid ? bias_before : bias_token[i - 1]) == id)) continue;
-        float x = Logit<T>::one(i == tid ? &bias_x : logits + n);
-        for (int32_t j = i; j < biases && bias_token[j] == id; ++j) x = __fadd_rn(x, bias_value[j]);
-        rules(n, counts[rank(n)], x);
+      if (biases > 0) named_sync(1, kChooseTableThreads);
+      for (int32_t i = tid; i < biases; i += kChooseTableThreads) {   // entries of one token add up
+        const int32_t id = bias_token[i];
+        const uint32_t n = here(id);
+        if (n >= static_cast<uint32_t>(width) || (i > 0 && bias_token[i - 1] == id)) continue;
+        const float *const value = a.bias_value + row * a.bias_stride;
+        float x = Logit<T>::one(logits + n);
+        for (int32_t j = i; j < biases && bias_token[j] == id; ++j) x = __fadd_rn(x, value[j]);
+        rules(n, rank(n), x);
       }
+    }
+    if (tid == 0) shared_listed = listed;
+  } else if (active) {
+    // -- the stream: every token as if the rules left it --
+    const int32_t me = tid - kChooseTableThreads;
+    float worst = -INFINITY;   // NaN and +inf stay in it: no rule makes them finite
+    if (vectors > 0) {
+      uint4 ahead[kChooseAhead];
+      uint32_t open[kChooseAhead], open_next[kChooseAhead];   // their mask words, as loaded
+      auto run = [&](auto mask_flag, auto out_flag) {
+        constexpr bool kMask = decltype(mask_flag)::value, kOut = decltype(out_flag)::value;
+        // Nothing here waits for a load; a step past the end fetches the slice's last
+        // vector again, for a load under a condition would be waited for.
+        auto fetch = [&](int k, int32_t step) {
+          const int32_t i = min(step * kChooseStreamThreads + me, vectors - 1);
+          ahead[k] = stream[i];
+          if (kMask) {
+            const int32_t w = (lead + i * kVec) >> 5;
+            open[k] = allowed[w];
+            if (split) open_next[k] = allowed[min(w + 1, last_word)];
+          }
+        };
+        const bool out16 = (reinterpret_cast<uintptr_t>(out + lead) & 15) == 0;
+        const int shift = (lead + me * kVec) & 31;   // a step is a whole number of mask words
+#pragma unroll
+        for (int k = 0; k < kChooseAhead; ++k) fetch(k, k);
+        for (int32_t step0 = 0; step0 < steps; step0 += kChooseAhead) {
+#pragma unroll
+          for (int k = 0; k < kChooseAhead; ++k) {
+            const int32_t step = step0 + k, vector = step * kChooseStreamThreads + me;
+            float x[kVec];
+            Logit<T>::unpack(ahead[k], x);
+            if (kMask) masked(x, split ? __funnelshift_r(open[k], open_next[k], shift) : open[k] >> shift);
+            fetch(k, step + kChooseAhead);
+            if (vector < vectors) {
+              if (kOut) {
+                float *const to = out + lead + vector * kVec;
+                if (out16) {
+#pragma unroll
+                  for (int j = 0; j < kVec; j += 4)
+                    __stcs(reinterpret_cast<float4 *>(to + j), make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]));
+                } else {
+#pragma unroll
+                  for (int j = 0; j < kVec; ++j) to[j] = x[j];
+                }
+              }
+              float here_top = x[0];
+#pragma unroll
+              for (int j = 1; j < kVec; ++j) here_top = max_nan(here_top, x[j]);
+              worst = max_nan(worst, here_top);
+              if (here_top > top) {   // a later equal one loses
+                top = here_top;
+#pragma unroll
+                for (int j = kVec - 1; j >= 0; --j)   // the first of the vector's equal ones
+                  if (x[j] == here_top) top_at = lead + vector * kVec + j;
+              }
+            }
+          }
+        }
+      };
+      using Yes = std::true_type;
+      using No = std::false_type;
+      static_assert(kChooseStreamThreads * kVec % 32 == 0, "a step is a whole number of mask words");
+      if (allowed != nullptr)
+        out != nullptr ? run(Yes{}, Yes{}) : run(Yes{}, No{});
+      else
+        out != nullptr ? run(No{}, Yes{}) : run(No{}, No{});
+    }
+    if (!(worst < INFINITY)) best.bad = 1;
+  }
+  // the tokens outside the vectors, a thread each
+  const int32_t single = tid < lead ? tid : tid - lead < width - rest ? rest + tid - lead : -1;
+  float single_x = -INFINITY;
+  if (active && single >= 0) {
+    single_x = open_at(single) ? Logit<T>::one(logits + single) : -INFINITY;
+    if (out != nullptr) out[single] = single_x;
+    if (!(single_x < INFINITY)) best.bad = 1;
+  }
+  __syncthreads();
+
+  if (active) {
+    const int32_t listed = shared_listed;
+    auto ruled = [&](int32_t n) { return listed > 0 && ((marks[n >> 5] >> (n & 31)) & 1u); };
+    // raises (value, at) to the first maximum of a vector's tokens that no rule is for
+    auto look = [&](int32_t vector, float &value, int32_t &at) {
+      float x[kVec];
+      Logit<T>::unpack(stream[vector], x);
+      const int32_t n = lead + vector * kVec;
+      if (allowed != nullptr)
+        masked(x, __funnelshift_r(allowed[n >> 5], allowed[min((n >> 5) + 1, last_word)], n & 31));
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        if (x[j] > value && !ruled(n + j)) {
+          value = x[j];
+          at = n + j;
+        }
+      }
+    };
+    const bool retake = top_at >= 0 && ruled(top_at);
+    if (retake) {
+      top = -INFINITY;
+      retake_list[atomicAdd(&retakes, 1)] = static_cast<uint16_t>(tid - kChooseTableThreads);
+    }
+    if (__syncthreads_or(retake)) {
+      const int32_t again = retakes;
+      constexpr int kWarps = kChooseThreads / 32;
+      if ((again + kWarps - 1) / kWarps * ((steps + 31) / 32) <= steps) {   // few: a warp takes a thread's elements together
+        for (int32_t q = tid >> 5; q < again; q += kWarps) {
+          float value = -INFINITY;
+          int32_t at = 0;
+          for (int32_t vector = (tid & 31) * kChooseStreamThreads + retake_list[q]; vector < vectors; vector += 32 * kChooseStreamThreads)
+            look(vector, value, at);
+          if (value > -INFINITY) better(best, value, v0 + at);
+        }
+      } else if (retake) {
+        for (int32_t vector = tid - kChooseTableThreads; vector < vectors; vector += kChooseStreamThreads) look(vector, top, top_at);
+      }
+    }
+    if (top > -INFINITY) better(best, top, v0 + top_at);
+    if (single_x > -INFINITY && !ruled(single)) better(best, single_x, v0 + single);
+
+    if (out != nullptr && listed > 0) {
+      // in place, the second look above has to end before a value replaces a logit
+      if (static_cast<const void *>(a.processed) == a.logits) __syncthreads();
+      for (int32_t i = tid; i < listed; i += kChooseThreads) out[list[i]] = __uint_as_float(counts[i]);
     }
   }
 
   best = warp_best(best);
   if ((tid & 31) == 0) warp_part[tid >> 5] = best;
   __syncthreads();
-  cluster_wait();
+  if (ctas > 1) cluster_wait();
   if (tid < 32) {
     best = tid < kChooseThreads / 32 ? warp_part[tid] : ChooseBest{-INFINITY, INT_MAX, 0};
     best = warp_best(best);
-    if (tid == 0) {
+    if (tid == 0 && ctas > 1) {
       store_cluster(&parts[part].value, 0, __float_as_uint(best.value));
       store_cluster(&parts[part].index, 0, static_cast<uint32_t>(best.index));
       store_cluster(&parts[part].bad, 0, static_cast<uint32_t>(best.bad));
     }
   }
-  cluster_arrive();
-  cluster_wait();
+  if (ctas > 1) {
+    cluster_arrive();
+    cluster_wait();
+    if (part == 0 && tid < 32) best = warp_best(tid < ctas ? parts[tid] : ChooseBest{-INFINITY, INT_MAX, 0});
+  }
   if (part == 0 && tid == 0) {
-    best = parts[0];
-    for (int c = 1; c < ctas; ++c) {
-      better(best, parts[c].value, parts[c].index);
-      best.bad |= parts[c].bad;
-    }
     const int64_t token = !active ? -1 : best.bad ? -2 : best.index == INT_MAX ? -1 : best.index;
     a.token[row] = token;
     if (a.append && a.history != nullptr && token >= 0) {

@@ -88,8 +88,8 @@ cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, 
 
 template <typename T, int D>
 cudaError_t rotate_typed(const RotateArgs &a, int device, cudaStream_t stream) {
-  constexpr int kHeads = 512 / D;   // heads a warp moves per round
-  const int all = (a.nq + 2 * a.nkv + kHeads - 1) / kHeads;
+  constexpr int kHeads = 512 / D;   // heads of a kind a warp moves per round
+  const int all = (a.nq + kHeads - 1) / kHeads + 2 * ((a.nkv + kHeads - 1) / kHeads);
   // as many rounds per warp as still leave 16 warps per SM: few tokens spread
   // their heads over the GPU, many keep their table row in registers
   const int64_t want = static_cast<int64_t>(sm_count(device)) * 16;
@@ -97,7 +97,10 @@ cudaError_t rotate_typed(const RotateArgs &a, int device, cudaStream_t stream) {
   const int warps_per_token = (all + rounds - 1) / rounds;
   const int64_t warps = static_cast<int64_t>(a.tokens) * warps_per_token;
   const unsigned grid = static_cast<unsigned>((warps * 32 + kRotateThreads - 1) / kRotateThreads);
-  rotate_store_kernel<T, D><<<grid, kRotateThreads, 0, stream>>>(a, rounds, warps_per_token);
+  if (a.q_norm != nullptr)
+    rotate_store_kernel<T, D, true><<<grid, kRotateThreads, 0, stream>>>(a, rounds, warps_per_token);
+  else
+    rotate_store_kernel<T, D, false><<<grid, kRotateThreads, 0, stream>>>(a, rounds, warps_per_token);
   return cudaGetLastError();
 }
 
@@ -194,8 +197,7 @@ cudaError_t choose_typed(const ChooseArgs &a, int device, cudaStream_t stream) {
     ctas *= 2;
   const int32_t slice = choose_slice(a.vocab, ctas);
   static std::atomic<uint64_t> done{0};
-  cudaError_t err = allow_shared(choose_kernel<T>, choose_shared(choose_slice(kChooseMaxVocab, kChooseMaxCluster), kMaxIndex),
-                                 device, done, true);
+  cudaError_t err = allow_shared(choose_kernel<T>, kChooseShared, device, done, true);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
@@ -419,6 +421,10 @@ int32_t cruise_decoder_choose(const void *logits, int64_t logits_stride, int32_t
   const char *const op = "cruise_decoder_choose";
   if (rows < 0 || rows > 65535 || vocab < 1 || vocab > kChooseMaxVocab)
     return refuse("%s: %d rows of %d logits (at most 65535 rows of 1 to %d)", op, rows, vocab, kChooseMaxVocab);
+  const int64_t entries = (history != nullptr ? history_width : 0) + static_cast<int64_t>(bias_token != nullptr ? bias_width : 0);
+  if (choose_shared(choose_slice(vocab, kChooseMaxCluster), entries) > kChooseShared)
+    return refuse("%s: a history and bias list of %lld entries with %d logits (at most 20000 beyond 390000 logits)", op,
+                  static_cast<long long>(entries), vocab);
   if (dtype < kBf16 || dtype > kFp32) return refuse("%s: dtype %d (0 bf16, 1 fp16 or 2 fp32)", op, dtype);
   if (logits_stride < vocab || (processed != nullptr && processed_stride < vocab) ||
       (allowed != nullptr && allowed_stride < (vocab + 31) / 32))

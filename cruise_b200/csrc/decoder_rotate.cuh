@@ -64,34 +64,40 @@ __device__ __forceinline__ void table8(const void *table, int32_t type, int64_t 
 // A lane holds two 16-byte chunks of a head: a chunk of the rotated part's
 // first half and its partner half a rotation further (or two neighbours behind
 // the rotated part), so the rotation needs no exchange between lanes.  D / 16
-// lanes share a head, a warp moves 512 / D heads of one token per round and
-// takes `rounds` rounds.  Norm weights and table entries become one factor per
-// element, z_lo = inv (x_lo c_lo + x_hi s_lo), kept in registers over the
-// token's heads.  kRotateBatch rounds of loads are in flight before their first use.
-template <typename T, int D>
+// lanes share a head, a warp moves 512 / D heads of one token and one kind (q,
+// k or v) per round and takes `rounds` rounds of the token's.  Norm weights and
+// table entries become one factor per element, z_lo = inv (x_lo c_lo + x_hi s_lo),
+// kept in registers over the token's heads.  kRotateBatch rounds of loads are in
+// flight before their first use.
+template <typename T, int D, bool Norm>
 __global__ void __launch_bounds__(kRotateThreads) rotate_store_kernel(const RotateArgs a, int rounds, int warps_per_token) {
   constexpr int kLanes = D / 16;
   constexpr int kHeads = 32 / kLanes;
   const int64_t warp = (static_cast<int64_t>(blockIdx.x) * kRotateThreads + threadIdx.x) >> 5;
   const int64_t t = warp / warps_per_token;
   if (t >= a.tokens) return;   // uniform over the warp
-  const int first = static_cast<int>(warp - t * warps_per_token) * rounds * kHeads;
   const int lane = threadIdx.x & 31;
   const int j = lane % kLanes, sub = lane / kLanes;
   const int half = a.rotary / 16;   // chunks in half the rotated part
   const bool turns = j < half;
-  const int lo = (turns ? j : 2 * j) * 8, hi = lo + (turns ? half : 1) * 8;   // this lane's elements of a head
-  const int last = min(a.nq + 2 * a.nkv, first + rounds * kHeads);
-  const T *src = static_cast<const T *>(a.qkv) + t * a.qkv_stride;
+  const int lo = (turns ? j : 2 * j) * 8, step = (turns ? half : 1) * 8;   // this lane's elements of a head: lo, lo + step
+  const int q_rounds = (a.nq + kHeads - 1) / kHeads, k_rounds = (a.nkv + kHeads - 1) / kHeads;
+  const int first = static_cast<int>(warp - t * warps_per_token) * rounds;
+  const int last = min(q_rounds + 2 * k_rounds, first + rounds);
+  const T *src = static_cast<const T *>(a.qkv) + t * a.qkv_stride + lo;
+  // of round r: its kind (0 q, 1 k, 2 v) and this lane's head of that kind
+  auto kind_of = [&](int r) { return r < q_rounds ? 0 : r < q_rounds + k_rounds ? 1 : 2; };
+  auto head_of = [&](int r, int kind) { return (r - (kind == 0 ? 0 : kind == 1 ? q_rounds : q_rounds + k_rounds)) * kHeads + sub; };
   uint4 raw[kRotateBatch][2];
-  auto load = [&](int base) {
+  auto load = [&](int r0) {
 #pragma unroll
-    for (int k = 0; k < kRotateBatch; ++k) {
-      const int head = base + k * kHeads + sub;
-      raw[k][0] = raw[k][1] = make_uint4(0, 0, 0, 0);
-      if (head < last) {
-        raw[k][0] = *reinterpret_cast<const uint4 *>(src + head * D + lo);
-        raw[k][1] = *reinterpret_cast<const uint4 *>(src + head * D + hi);
+    for (int b = 0; b < kRotateBatch; ++b) {
+      const int r = r0 + b, kind = kind_of(r), head = head_of(r, kind);
+      raw[b][0] = raw[b][1] = make_uint4(0, 0, 0, 0);
+      if (r < last && head < (kind == 0 ? a.nq : a.nkv)) {
+        const T *x = src + ((kind == 0 ? 0 : kind == 1 ? a.nq : a.nq + a.nkv) + head) * D;
+        raw[b][0] = *reinterpret_cast<const uint4 *>(x);
+        raw[b][1] = *reinterpret_cast<const uint4 *>(x + step);
       }
     }
   };
@@ -100,69 +106,54 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_store_kernel(const Rota
   const int32_t slot = a.slot[t];
   const bool known = pos >= 0 && pos < a.rope_rows;
   const bool stored = known && slot >= 0 && slot < a.num_blocks * a.block_size;
-  const bool norm = a.q_norm != nullptr;
-  T *q_dst = static_cast<T *>(a.q_out) + t * a.q_stride;
-  const int64_t cell = stored ? (slot / a.block_size) * a.block_stride + static_cast<int64_t>(slot % a.block_size) * a.nkv * D : 0;
-  T *k_dst = static_cast<T *>(a.key_cache) + cell;
-  T *v_dst = static_cast<T *>(a.value_cache) + cell;
+  T *q_dst = static_cast<T *>(a.q_out) + t * a.q_stride + lo;
+  const int64_t cell =
+      (stored ? (slot / a.block_size) * a.block_stride + static_cast<int64_t>(slot % a.block_size) * a.nkv * D : 0) + lo;
   // z_lo = x_lo c_lo + x_hi s_lo, z_hi = x_hi c_hi + x_lo s_hi (times the head's inverse norm)
   float2 c_lo[4], c_hi[4], s_lo[4], s_hi[4];
-  int built = -1;   // whose factors the lane holds: 0 query heads, 1 key heads
-  for (int base = first; base < last; base += kRotateBatch * kHeads) {
-    if (base > first) load(base);
+  auto factors = [&](const void *weights) {
 #pragma unroll
-    for (int k = 0; k < kRotateBatch; ++k) {
-      const int begin = base + k * kHeads, head = begin + sub;
-      if (begin >= last) break;   // uniform over the warp
-      if (begin < a.nq + a.nkv) {
-        const int kind = norm && head >= a.nq ? 1 : 0;
-        if (built != kind) {
+    for (int i = 0; i < 4; ++i) {
+      c_lo[i] = c_hi[i] = make_float2(1.f, 1.f);
+      s_lo[i] = s_hi[i] = make_float2(0.f, 0.f);
+    }
+    if (known && turns) {
+      const int64_t at = pos * a.rotary + lo;
+      table8(a.rope_cos, a.rope_dtype, at, c_lo);
+      table8(a.rope_cos, a.rope_dtype, at + step, c_hi);
+      table8(a.rope_sin, a.rope_dtype, at, s_lo);
+      table8(a.rope_sin, a.rope_dtype, at + step, s_hi);
+    }
+    if (Norm) {
+      float2 w_lo[4], w_hi[4];
+      unpack2<T>(*reinterpret_cast<const uint4 *>(static_cast<const T *>(weights) + lo), w_lo);
+      unpack2<T>(*reinterpret_cast<const uint4 *>(static_cast<const T *>(weights) + lo + step), w_hi);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            c_lo[i] = c_hi[i] = make_float2(1.f, 1.f);
-            s_lo[i] = s_hi[i] = make_float2(0.f, 0.f);
-          }
-          if (known && turns) {
-            table8(a.rope_cos, a.rope_dtype, pos * a.rotary + lo, c_lo);
-            table8(a.rope_cos, a.rope_dtype, pos * a.rotary + hi, c_hi);
-            table8(a.rope_sin, a.rope_dtype, pos * a.rotary + lo, s_lo);
-            table8(a.rope_sin, a.rope_dtype, pos * a.rotary + hi, s_hi);
-          }
-          if (norm) {
-            const T *weight = static_cast<const T *>(kind == 0 ? a.q_norm : a.k_norm);
-            float2 w_lo[4], w_hi[4];
-            unpack2<T>(*reinterpret_cast<const uint4 *>(weight + lo), w_lo);
-            unpack2<T>(*reinterpret_cast<const uint4 *>(weight + hi), w_hi);
+      for (int i = 0; i < 4; ++i) {
+        c_lo[i] = mul2(c_lo[i], w_lo[i]);
+        c_hi[i] = mul2(c_hi[i], w_hi[i]);
+        s_lo[i] = mul2(s_lo[i], w_hi[i]);
+        s_hi[i] = mul2(s_hi[i], w_lo[i]);
+      }
+    }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              c_lo[i] = mul2(c_lo[i], w_lo[i]);
-              c_hi[i] = mul2(c_hi[i], w_hi[i]);
-              s_lo[i] = mul2(s_lo[i], w_hi[i]);
-              s_hi[i] = mul2(s_hi[i], w_lo[i]);
-            }
-          }
+    for (int i = 0; i < 4; ++i) s_lo[i] = make_float2(-s_lo[i].x, -s_lo[i].y);
+  };
+  int built = kind_of(first);
+  if (built < 2) factors(built == 0 ? a.q_norm : a.k_norm);
+  for (int r0 = first; r0 < last; r0 += kRotateBatch) {
+    if (r0 > first) load(r0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s_lo[i] = make_float2(-s_lo[i].x, -s_lo[i].y);
-          built = kind;
-        }
-        float2 x_lo[4], x_hi[4];
-        unpack2<T>(raw[k][0], x_lo);
-        unpack2<T>(raw[k][1], x_hi);
-        float inv = 1.f;
-        if (norm) {
-          float2 ss = make_float2(0.f, 0.f);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            ss = fma2(x_lo[i], x_lo[i], ss);
-            ss = fma2(x_hi[i], x_hi[i], ss);
-          }
-          float sum = ss.x + ss.y;
-#pragma unroll
-          for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          inv = rsqrtf(sum * (1.f / D) + a.eps);
-        }
-        const float2 inv2 = make_float2(inv, inv);
-        float2 z_lo[4], z_hi[4];
+    for (int b = 0; b < kRotateBatch; ++b) {
+      const int r = r0 + b;
+      if (r >= last) break;
+      const int kind = kind_of(r), head = head_of(r, kind);   // the kind is uniform over the warp
+      if (kind < 2) {
+        if (Norm && kind != built) factors(a.k_norm);
+        built = kind;
+        float2 x_lo[4], x_hi[4], z_lo[4], z_hi[4];
+        unpack2<T>(raw[b][0], x_lo);
+        unpack2<T>(raw[b][1], x_hi);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           z_lo[i] = mul2(x_lo[i], c_lo[i]);
@@ -171,20 +162,38 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_store_kernel(const Rota
             z_lo[i] = fma2(x_hi[i], s_lo[i], z_lo[i]);
             z_hi[i] = fma2(x_lo[i], s_hi[i], z_hi[i]);
           }
-          z_lo[i] = mul2(z_lo[i], inv2);
-          z_hi[i] = mul2(z_hi[i], inv2);
         }
-        if (head < a.nq + a.nkv) {
-          raw[k][0] = pack2<T>(z_lo);
-          raw[k][1] = pack2<T>(z_hi);
+        if (Norm) {
+          float2 s0 = mul2(x_lo[0], x_lo[0]), s1 = mul2(x_hi[0], x_hi[0]);
+#pragma unroll
+          for (int i = 1; i < 4; ++i) {
+            s0 = fma2(x_lo[i], x_lo[i], s0);
+            s1 = fma2(x_hi[i], x_hi[i], s1);
+          }
+          float sum = (s0.x + s0.y) + (s1.x + s1.y);
+#pragma unroll
+          for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          const float inv = rsqrtf(sum * (1.f / D) + a.eps);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            z_lo[i] = mul2(z_lo[i], make_float2(inv, inv));
+            z_hi[i] = mul2(z_hi[i], make_float2(inv, inv));
+          }
         }
+        raw[b][0] = pack2<T>(z_lo);
+        raw[b][1] = pack2<T>(z_hi);
       }
-      if (head >= last) continue;
-      if (head < a.nq && !known) raw[k][0] = raw[k][1] = make_uint4(0, 0, 0, 0);
-      if (head >= a.nq && !stored) continue;
-      T *dst = head < a.nq ? q_dst + head * D : head < a.nq + a.nkv ? k_dst + (head - a.nq) * D : v_dst + (head - a.nq - a.nkv) * D;
-      *reinterpret_cast<uint4 *>(dst + lo) = raw[k][0];
-      *reinterpret_cast<uint4 *>(dst + hi) = raw[k][1];
+      if (kind == 0) {
+        if (head < a.nq) {
+          T *dst = q_dst + head * D;
+          *reinterpret_cast<uint4 *>(dst) = known ? raw[b][0] : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4 *>(dst + step) = known ? raw[b][1] : make_uint4(0, 0, 0, 0);
+        }
+      } else if (stored && head < a.nkv) {
+        T *dst = static_cast<T *>(kind == 1 ? a.key_cache : a.value_cache) + cell + head * D;
+        *reinterpret_cast<uint4 *>(dst) = raw[b][0];
+        *reinterpret_cast<uint4 *>(dst + step) = raw[b][1];
+      }
     }
   }
 }

@@ -104,7 +104,8 @@ int64_t cruise_decoder_attention_workspace(int32_t rows, int32_t num_heads,
  * same stride), else must not overlap them.  append: token[r] >= 0 is written to
  * history[r][history_len[r]] where that is inside history_width (history_len
  * itself is the caller's to advance).  4-byte alignment suffices (logits: their
- * own size).  vocab at most 393216. */
+ * own size).  vocab at most 2^20; beyond
+ * 390000 at most 20000 history and bias entries together. */
 int32_t cruise_decoder_choose(
     const void *logits, int64_t logits_stride, int32_t rows, int32_t vocab,
     int32_t dtype, const int32_t *active, int32_t *history,

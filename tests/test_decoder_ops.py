@@ -73,7 +73,8 @@ def test_attention_refuses(change, reason):
 
 
 @pytest.mark.parametrize("change, reason", [
-    (dict(rows=-1), "rows"), (dict(rows=70000), "rows"), (dict(vocab=0), "logits"), (dict(vocab=393217), "logits"),
+    (dict(rows=-1), "rows"), (dict(rows=70000), "rows"), (dict(vocab=0), "logits"), (dict(vocab=(1 << 20) + 1), "logits"),
+    (dict(vocab=1000000, logits_stride=1000000, history_width=30000, history_stride=30000), "entries"),
     (dict(dtype=3), "dtype"), (dict(logits_stride=99), "stride"), (dict(history_width=11), "history"),
     (dict(history_len=None), "history"), (dict(history=None), "need a history"),
     (dict(history=None, append=0, presence=at(6)), "need a history"),
