@@ -24,12 +24,12 @@ constexpr int kAttendKeys = 16;      // keys of a warp's step
 constexpr int kAttendStages = 3;
 constexpr int kAttendWarps = 4;      // warps of a CTA that shares the work with the others
 constexpr int kAttendWholeWarps = 8; // warps of a CTA that takes one whole unit
-constexpr int kJoinThreads = 1024;
+constexpr int kJoinThreads = 512;
 constexpr int kJoinBatch = 6;        // pieces a thread has in flight
 
 // CTAs per SM that share the work: what shared memory (head size 128) or
-// registers allow.
-__host__ __device__ constexpr int attend_ctas(int d, int nt) { return d == 128 ? 2 : nt == 1 ? 4 : 3; }
+// registers (64, for 16 heads a unit) allow.
+__host__ __device__ constexpr int attend_ctas(int d) { return d == 128 ? 2 : 3; }
 
 // What starting a unit costs, in tiles: the pipeline fills and the warps' parts
 // meet once per unit, whatever its length.
@@ -48,7 +48,11 @@ struct AttentionPlan {
   float scale_log2;    // scale * log2(e)
   float *piece_o;      // [2 grid][heads][d]
   float *piece_ml;     // [2 grid][heads][2]
-  int4 *piece_of;      // [grid]: row, unit, pieces of the unit that begins in the CTA's slot 1 (0: none)
+  // Where the join finds a split unit: row, unit, pieces (0: not split), the CTA of
+  // its first piece.  By unit [rows * units], written by the CTA that begins it, or
+  // where units outnumber the CTAs by CTA [grid], for the unit in its slot 1.
+  int4 *piece_of;
+  int32_t by_unit;
 };
 
 template <int D, int Warps>
@@ -97,7 +101,7 @@ __host__ __device__ __forceinline__ int row_tiles(int length) {
 }
 
 template <typename T, int D, int NT, int Warps, bool Whole>
-__global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D, NT)) attention_kernel(const AttentionPlan p) {
+__global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attention_kernel(const AttentionPlan p) {
   using S = AttendShared<D, Warps>;
   constexpr int kAttendThreads = Warps * 32, kAttendTile = Warps * kAttendKeys;
   extern __shared__ __align__(128) uint8_t ring[];
@@ -143,7 +147,7 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D, NT)) at
     const int share = max(2 * kSetup, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
     const int64_t begin64 = static_cast<int64_t>(blockIdx.x) * share;
     if (begin64 >= total) {
-      if (tid == 0) p.piece_of[blockIdx.x] = make_int4(0, 0, 0, 0);
+      if (!p.by_unit && tid == 0) p.piece_of[blockIdx.x] = make_int4(0, 0, 0, 0);
       return;
     }
     const int begin = static_cast<int>(begin64);
@@ -391,16 +395,23 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D, NT)) at
       }
     }
     __syncthreads();   // the ring is free for the next segment
-    if (!whole && t0 == 0) tail = make_int4(row_now, unit, 1 + (n - count + share_work - 1) / share_work, 0);
+    if (!Whole && t0 == 0) {
+      const int4 of = make_int4(row_now, unit, whole ? 0 : 1 + (n - count + share_work - 1) / share_work, blockIdx.x);
+      if (p.by_unit) {
+        if (tid == 0) p.piece_of[row_now * p.units + unit] = of;
+      } else if (!whole) {
+        tail = of;
+      }
+    }
   }
-  if (!Whole && tid == 0) p.piece_of[blockIdx.x] = tail;
+  if (!Whole && !p.by_unit && tid == 0) p.piece_of[blockIdx.x] = tail;
 }
 
-// Joins the pieces of the unit that begins in CTA blockIdx.x of the attention
-// and goes on after it.  D / 4 lanes take a head's row of a piece, four
-// dimensions each; the lanes' groups share the heads and their pieces.
+// Joins the pieces of a split unit (piece_of), `heads_each` of its heads a CTA.
+// D / 4 lanes take a head's row of a piece, four dimensions each; the lanes'
+// groups share the heads and their pieces.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kJoinThreads, 1) attention_join_kernel(const AttentionPlan p) {
+__global__ void __launch_bounds__(kJoinThreads, 1) attention_join_kernel(const AttentionPlan p, const int32_t heads_each) {
   constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
   __shared__ __align__(16) float red[kGroups][D];
   __shared__ float red_ml[kGroups][2];
@@ -410,8 +421,11 @@ __global__ void __launch_bounds__(kJoinThreads, 1) attention_join_kernel(const A
   if (pieces == 0) return;
   const AttentionArgs &a = p.a;
   const int row = of.x, kvh = of.y / p.chunks;
-  const int head0 = kvh * p.groups + (of.y - kvh * p.chunks) * p.chunk;
-  const int heads = min(p.chunk, (kvh + 1) * p.groups - head0);
+  const int unit_head0 = kvh * p.groups + (of.y - kvh * p.chunks) * p.chunk;
+  const int skip = blockIdx.y * heads_each;   // the unit's heads before this CTA's
+  const int head0 = unit_head0 + skip;
+  const int heads = min(min(p.chunk, (kvh + 1) * p.groups - unit_head0) - skip, heads_each);
+  if (heads <= 0) return;
   const int parts = min(kGroups / heads, pieces);   // groups that share a head
   const int c = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const int h = group % heads, part = group / heads;
@@ -428,9 +442,9 @@ __global__ void __launch_bounds__(kJoinThreads, 1) attention_join_kernel(const A
         v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (i < pieces) {
           // the first piece lies in slot 1 of its CTA, the others in slot 0 of the CTAs after it
-          const int64_t piece = i == 0 ? 2 * static_cast<int64_t>(blockIdx.x) + 1 : 2 * (static_cast<int64_t>(blockIdx.x) + i);
-          ml[k] = *reinterpret_cast<const float2 *>(p.piece_ml + (piece * (NT * 8) + h) * 2);
-          v[k] = *reinterpret_cast<const float4 *>(p.piece_o + piece * (NT * 8 * D) + h * D + c * 4);
+          const int64_t piece = i == 0 ? 2 * static_cast<int64_t>(of.w) + 1 : 2 * (static_cast<int64_t>(of.w) + i);
+          ml[k] = *reinterpret_cast<const float2 *>(p.piece_ml + (piece * (NT * 8) + skip + h) * 2);
+          v[k] = *reinterpret_cast<const float4 *>(p.piece_o + piece * (NT * 8 * D) + (skip + h) * D + c * 4);
         }
       }
       float top = m;

@@ -123,7 +123,7 @@ AttentionShape attention_shape(int32_t rows, int32_t nq, int32_t nkv, int32_t d,
   // few short rows: one CTA per unit and no second kernel
   const int sms = sm_count(device);
   s.whole = capacity <= 4 * kAttendWholeWarps * kAttendKeys && static_cast<int64_t>(rows) * s.units <= sms;
-  s.grid = sms * attend_ctas(d, s.chunk <= 8 ? 1 : 2);
+  s.grid = sms * attend_ctas(d);
   return s;
 }
 
@@ -159,6 +159,7 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
     kernel<<<static_cast<unsigned>(a.rows) * s.units, kAttendWholeWarps * 32, smem, stream>>>(p);
     return cudaGetLastError();
   }
+  p.by_unit = static_cast<int64_t>(a.rows) * s.units <= s.grid ? 1 : 0;
   size_t ml = 0, of = 0;
   pieces_bytes(s.grid, NT * 8, D, &ml, &of);
   uint8_t *w = static_cast<uint8_t *>(a.workspace);
@@ -172,7 +173,11 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
   kernel<<<s.grid, kAttendWarps * 32, smem, stream>>>(p);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
-  return launch_dependent(attention_join_kernel<T, D, NT>, dim3(s.grid), kJoinThreads, stream, p);
+  // few units: a CTA for some heads of each, so that the join is spread over the SMs
+  const int64_t units = static_cast<int64_t>(a.rows) * s.units;
+  const int entries = p.by_unit ? static_cast<int>(units) : s.grid;
+  const int each = std::clamp((s.chunk * entries + sm_count(device) - 1) / sm_count(device), 1, s.chunk);
+  return launch_dependent(attention_join_kernel<T, D, NT>, dim3(entries, (s.chunk + each - 1) / each), kJoinThreads, stream, p, each);
 }
 
 template <typename T>

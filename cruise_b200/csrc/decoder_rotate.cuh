@@ -15,6 +15,7 @@ namespace cruise {
 namespace ops {
 
 constexpr int kRotateThreads = 128;
+constexpr int kRotateCtas = 5;    // CTAs per SM
 constexpr int kRotateBatch = 3;
 
 // Two fp32 operations in one instruction.
@@ -70,7 +71,7 @@ __device__ __forceinline__ void table8(const void *table, int32_t type, int64_t 
 // kept in registers over the token's heads.  kRotateBatch rounds of loads are in
 // flight before their first use.
 template <typename T, int D, bool Norm>
-__global__ void __launch_bounds__(kRotateThreads) rotate_store_kernel(const RotateArgs a, int rounds, int warps_per_token) {
+__global__ void __launch_bounds__(kRotateThreads, kRotateCtas) rotate_store_kernel(const RotateArgs a, int rounds, int warps_per_token) {
   constexpr int kLanes = D / 16;
   constexpr int kHeads = 32 / kLanes;
   const int64_t warp = (static_cast<int64_t>(blockIdx.x) * kRotateThreads + threadIdx.x) >> 5;
