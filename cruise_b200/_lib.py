@@ -83,6 +83,10 @@ SIGNATURES = {
         ctypes.c_int32,
         [ctypes.c_void_p, i64p, i64p, i32p, ctypes.c_void_p, i32p, i32p, i32p, ctypes.c_void_p, u8p, f32p, i64p],
     ),
+    "cruise_decoder_step_paged": (
+        ctypes.c_int32,
+        [_ptr, _i32, _ptr, _ptr, _ptr, _ptr, _i64, _i32, _ptr, _i64, _i32, _ptr, _ptr, _i32, _i32, _ptr, _i64, _ptr],
+    ),
     "cruise_epoch_last_timing": (
         ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_double), i32p]
     ),

@@ -22,6 +22,7 @@
 #include <vector>
 
 #include "../../include/cruise_epoch.h"
+#include "decoder_ops.h"
 #include "epoch_kernel.cuh"
 #include "prefill.cuh"
 #include "prefill_gemm.cuh"
@@ -187,6 +188,18 @@ struct PrefillState {
 };
 constexpr int kTraceLaunches = 8;
 
+// Buffers of the decoder step over caller-held paged caches, beside the
+// prefill's, built on the first cruise_decoder_step_paged.
+struct PagedState {
+  void *work = nullptr;
+  bf16 *qkv = nullptr;           // [max_tokens][Nqkv]
+  bf16 *logits = nullptr;        // [max_tokens][V_pad]
+  int32_t *slot = nullptr, *length = nullptr;
+  void *attention = nullptr;     // the attention's workspace
+  int64_t attention_bytes = 0;
+  cudaEvent_t before = nullptr, after = nullptr;   // the caller's stream and the engine's, one after the other
+};
+
 struct Engine {
   CruiseModelConfig cfg{};
   ModelDims m{};
@@ -241,6 +254,7 @@ struct Engine {
   StreamRing *d_stream = nullptr;          // its device view
   bool stream_on = false;
   PrefillState *prefill = nullptr;
+  PagedState *paged = nullptr;
   bool payload_ready = false;   // d_payload holds a prefilled cohort for the next import epoch
   uint64_t tp_timeout_ns = 20000000000ull;   // device waits on other ranks (CRUISE_TP_TIMEOUT_MS)
 };
@@ -386,6 +400,7 @@ void default_rope(const Engine *e, std::vector<uint16_t> &cos_t, std::vector<uin
 }
 
 void prefill_release(Engine *e);
+void paged_release(Engine *e);
 
 void destroy_engine(Engine *e) {
   if (e == nullptr) return;
@@ -402,6 +417,7 @@ void destroy_engine(Engine *e) {
   if (e->h_io) cudaFreeHost(e->h_io);
   if (e->h_stream) cudaFreeHost(e->h_stream);
   prefill_release(e);
+  paged_release(e);
   if (e->ev0) cudaEventDestroy(e->ev0);
   if (e->ev1) cudaEventDestroy(e->ev1);
   if (e->stream) cudaStreamDestroy(e->stream);
@@ -1156,6 +1172,213 @@ int32_t prefill_run(Engine *e, const int64_t *tokens, const int32_t *lens, int32
   return 0;
 }
 
+void paged_release(Engine *e) {
+  PagedState *ps = e->paged;
+  if (ps == nullptr) return;
+  cudaFree(ps->work);
+  cudaFree(ps->attention);
+  if (ps->before) cudaEventDestroy(ps->before);
+  if (ps->after) cudaEventDestroy(ps->after);
+  delete ps;
+  e->paged = nullptr;
+}
+
+int32_t paged_prepare(Engine *e) {
+  if (e->paged != nullptr) return 0;
+  const ModelDims &m = e->m;
+  auto *ps = new PagedState();
+  e->paged = ps;
+  const size_t T = e->prefill->max_tokens;
+  size_t bytes = 0;
+  auto take = [&](size_t n) { const size_t off = bytes; bytes = align_up(bytes + n, 1024); return off; };
+  const size_t o_qkv = take(T * m.Nqkv * 2), o_logits = take(T * m.V_pad * 2), o_slot = take(T * 4), o_length = take(T * 4);
+  cudaError_t err = cudaMalloc(&ps->work, bytes);
+  if (err == cudaSuccess) err = cudaEventCreateWithFlags(&ps->before, cudaEventDisableTiming);
+  if (err == cudaSuccess) err = cudaEventCreateWithFlags(&ps->after, cudaEventDisableTiming);
+  if (err != cudaSuccess) return set_err(e, err, "paged decoder step buffers");
+  uint8_t *b = static_cast<uint8_t *>(ps->work);
+  ps->qkv = reinterpret_cast<bf16 *>(b + o_qkv);
+  ps->logits = reinterpret_cast<bf16 *>(b + o_logits);
+  ps->slot = reinterpret_cast<int32_t *>(b + o_slot);
+  ps->length = reinterpret_cast<int32_t *>(b + o_length);
+  return 0;
+}
+
+// What cruise_decoder_step_paged is given, checked.
+struct PagedStep {
+  int32_t rows;
+  const int64_t *token, *position;
+  bf16 *key_cache, *value_cache;
+  int64_t num_blocks;
+  int32_t block_size;
+  const int32_t *block_table;
+  int64_t table_stride;
+  int32_t table_width;
+  const void *rope_cos, *rope_sin;   // nullptr: the engine's tables
+  int32_t rope_dtype, rope_rows;
+  uint16_t *logits;
+  int64_t logits_stride;
+  cudaStream_t stream;
+};
+
+// One decoder step of `rows` rows layer by layer: the prefill's projections
+// and norms around rotate_store and paged_attention on the caller's caches.
+int32_t run_decoder_step_paged(Engine *e, const PagedStep &s) {
+  const ModelDims &m = e->m;
+  auto reject = [&](const std::string &why) {
+    e->last_error = "cruise_decoder_step_paged: " + why;
+    return -1;
+  };
+  if (e->tp_size > 1 || m.Kq != m.Hq) {
+    e->last_error = "cruise_decoder_step_paged: single-GPU engines only (no tensor parallelism)";
+    return -4;
+  }
+  if (m.I % 8 != 0 || m.H % 8 != 0 || m.H > 8 * prefill::kNormThreads * prefill::kNormChunks)
+    return reject("needs intermediate and hidden sizes divisible by 8 and a hidden size of at most 8192");
+  const int64_t capacity = static_cast<int64_t>(s.table_width) * s.block_size;
+  if (s.rows < 1 || s.rows > kBatch * m.bs) return reject("rows outside [1, 4 block_size]");
+  if (s.num_blocks < 1 || s.block_size < 1 || s.num_blocks > 0x7fffffff / s.block_size || s.table_width < 1 ||
+      s.table_stride < s.table_width || capacity > 0x40000000)
+    return reject("caches and tables need at least one block, below 2^31 slots and 2^30 positions a row");
+  if (static_cast<int64_t>(s.rows) * m.nkv * ((m.nq / m.nkv + 15) / 16) * (capacity / 64 + 8) > 0x7fffffff)
+    return reject("rows x KV heads x capacity / 64 passes 2^31");
+  if (s.logits_stride < m.V) return reject("the stride of the logits is smaller than the vocabulary");
+  if ((s.rope_cos == nullptr) != (s.rope_sin == nullptr)) return reject("pass both rotation tables or neither");
+  if (s.rope_cos != nullptr && ((s.rope_dtype != ops::kBf16 && s.rope_dtype != ops::kFp32) || s.rope_rows < 1))
+    return reject("rotation tables are bf16 (0) or fp32 (2) with at least one row");
+  for (const void *p : {static_cast<const void *>(s.key_cache), static_cast<const void *>(s.value_cache), s.rope_cos, s.rope_sin})
+    if ((reinterpret_cast<uintptr_t>(p) & 15) != 0) return reject("caches and tables must be 16-byte aligned");
+  for (const void *p : {static_cast<const void *>(s.token), static_cast<const void *>(s.position),
+                        static_cast<const void *>(s.key_cache), static_cast<const void *>(s.value_cache),
+                        static_cast<const void *>(s.block_table), static_cast<const void *>(s.logits)}) {
+    cudaPointerAttributes attr{};
+    if (cudaPointerGetAttributes(&attr, p) != cudaSuccess || attr.type != cudaMemoryTypeDevice || attr.device != e->device) {
+      cudaGetLastError();
+      return reject("every tensor must be device memory on the engine's device");
+    }
+  }
+  int32_t rc = prefill_prepare(e);
+  if (rc != 0) {
+    prefill_release(e);
+    return rc;
+  }
+  rc = paged_prepare(e);
+  if (rc != 0) {
+    paged_release(e);
+    return rc;
+  }
+  PrefillState *ps = e->prefill;
+  PagedState *pg = e->paged;
+  const int64_t need = ops::attention_workspace(s.rows, m.nq, m.nkv, m.d, capacity, e->device);
+  if (need > pg->attention_bytes) {   // the steps before have completed
+    cudaFree(pg->attention);
+    pg->attention = nullptr;
+    pg->attention_bytes = 0;
+    const cudaError_t err = cudaMalloc(&pg->attention, need);
+    if (err != cudaSuccess) return set_err(e, err, "paged attention workspace");
+    pg->attention_bytes = need;
+  }
+  const int T = s.rows, H = m.H, I = m.I, N = m.Nqkv;
+  const int32_t rope_rows = s.rope_cos != nullptr ? s.rope_rows : m.C;
+  cudaError_t err = cudaEventRecord(pg->before, s.stream);
+  if (err == cudaSuccess) err = cudaStreamWaitEvent(e->stream, pg->before, 0);
+  if (err == cudaSuccess) err = cudaMemsetAsync(ps->error, 0, 4, e->stream);
+  if (err != cudaSuccess) return set_err(e, err, "paged decoder step inputs");
+  const GemmPlan pq = gemm_plan(e, N, H, T), po = gemm_plan(e, H, m.Hq, T);
+  const GemmPlan pg_up = gemm_plan(e, 2 * I, H, T, false), pd = gemm_plan(e, H, m.I_pad, T);
+  const GemmPlan pv = gemm_plan(e, m.V_pad, H, T, false);
+  const unsigned parts_threads = static_cast<unsigned>(prefill::parts_norm_threads(H));
+  ops::RotateArgs ra{};
+  ra.qkv = pg->qkv;
+  ra.qkv_stride = N;
+  ra.tokens = T;
+  ra.nq = m.nq;
+  ra.nkv = m.nkv;
+  ra.d = m.d;
+  ra.dtype = ops::kBf16;
+  ra.position = s.position;
+  ra.slot = pg->slot;
+  ra.rope_cos = s.rope_cos != nullptr ? s.rope_cos : e->rope_cos;
+  ra.rope_sin = s.rope_cos != nullptr ? s.rope_sin : e->rope_sin;
+  ra.rope_dtype = s.rope_cos != nullptr ? s.rope_dtype : static_cast<int32_t>(ops::kBf16);
+  ra.rope_rows = rope_rows;
+  ra.rotary = m.d;
+  ra.q_out = ps->q;
+  ra.q_stride = m.Hq;
+  ra.num_blocks = s.num_blocks;
+  ra.block_size = s.block_size;
+  ra.block_stride = static_cast<int64_t>(s.block_size) * m.nkv * m.d;
+  ops::AttentionArgs aa{};
+  aa.q = ps->q;
+  aa.q_stride = m.Hq;
+  aa.rows = T;
+  aa.nq = m.nq;
+  aa.nkv = m.nkv;
+  aa.d = m.d;
+  aa.dtype = ops::kBf16;
+  aa.num_blocks = s.num_blocks;
+  aa.block_stride = ra.block_stride;
+  aa.block_size = s.block_size;
+  aa.block_table = s.block_table;
+  aa.table_stride = s.table_stride;
+  aa.table_width = s.table_width;
+  aa.seq_len = pg->length;
+  aa.scale = 1.f / m.sqrt_d;
+  aa.out = ps->attn;
+  aa.out_stride = m.Hq;
+  aa.workspace = pg->attention;
+  const int64_t layer_elems = s.num_blocks * ra.block_stride;
+  prefill::paged_rows<<<T, 128, 0, e->stream>>>(e->embed, s.token, s.position, s.block_table, s.table_stride, s.table_width,
+                                                s.block_size, s.num_blocks, rope_rows, m.V, ps->h, pg->slot, pg->length, H);
+  chain_launch(e, T, 256, 0, prefill::rms_norm_rows, ps->h, e->layers[0].w_in, ps->x, H, m.eps);
+  bool gemm_ok = true;
+  for (int l = 0; l < m.L && gemm_ok && err == cudaSuccess; ++l) {
+    // x holds rms_norm(h) * w_in of this layer
+    const LayerWeights &lw = e->layers[l];
+    gemm_ok &= prefill_gemm(e, lw.qkv_w, N, H, ps->x, T, H, 0, pq, nullptr);
+    chain_launch(e, dim3(T, (N / 2 + 255) / 256), 256, 0, prefill::qkv_bias_rows, ps->acc, pq.nsplit, T, lw.qkv_b, pg->qkv, N);
+    ra.key_cache = s.key_cache + l * layer_elems;
+    ra.value_cache = s.value_cache + l * layer_elems;
+    aa.key_cache = ra.key_cache;
+    aa.value_cache = ra.value_cache;
+    err = ops::launch_rotate_store(ra, e->device, e->stream);
+    if (err == cudaSuccess) err = ops::launch_paged_attention(aa, e->device, e->stream);
+    if (po.nsplit == 1) {
+      gemm_ok &= prefill_gemm(e, lw.o_w, H, m.Hq, ps->attn, T, m.Hq, 2, po, ps->y);
+      chain_launch(e, T, prefill::kNormThreads, 0, prefill::residual_rms_norm, ps->y, ps->h, lw.w_post, ps->x, H, m.eps);
+    } else {
+      gemm_ok &= prefill_gemm(e, lw.o_w, H, m.Hq, ps->attn, T, m.Hq, 0, po, nullptr);
+      chain_launch(e, T, parts_threads, 0, prefill::residual_rms_norm_parts, ps->acc, po.nsplit, T, ps->h, lw.w_post, ps->x, H,
+                   m.eps);
+    }
+    gemm_ok &= prefill_gemm(e, lw.gu_w, 2 * I, H, ps->x, T, H, 1, pg_up, ps->act);
+    gemm_ok &= prefill_gemm(e, lw.down_w, H, m.I_pad, ps->act, T, I, 0, pd, nullptr);
+    chain_launch(e, T, parts_threads, 0, prefill::residual_rms_norm_parts, ps->acc, pd.nsplit, T, ps->h,
+                 l + 1 < m.L ? e->layers[l + 1].w_in : e->final_norm, ps->x, H, m.eps);
+  }
+  if (gemm_ok && err == cudaSuccess) gemm_ok = prefill_gemm(e, e->lm_head, m.V_pad, H, ps->x, T, H, 2, pv, pg->logits);
+  if (!gemm_ok) {   // prefill_gemm left the reason in last_error
+    cudaStreamSynchronize(e->stream);
+    return -2;
+  }
+  if (err == cudaSuccess) err = cudaGetLastError();
+  if (err == cudaSuccess)
+    err = cudaMemcpy2DAsync(s.logits, s.logits_stride * 2, pg->logits, static_cast<size_t>(m.V_pad) * 2, static_cast<size_t>(m.V) * 2,
+                            T, cudaMemcpyDeviceToDevice, e->stream);
+  uint32_t site = 0;
+  if (err == cudaSuccess) err = cudaMemcpyAsync(&site, ps->error, 4, cudaMemcpyDeviceToHost, e->stream);
+  if (err == cudaSuccess) err = cudaEventRecord(pg->after, e->stream);
+  if (err == cudaSuccess) err = cudaStreamWaitEvent(s.stream, pg->after, 0);
+  const cudaError_t done = cudaStreamSynchronize(e->stream);   // (also after a failure: the buffers are free again)
+  if (err == cudaSuccess) err = done;
+  if (err != cudaSuccess) return set_err(e, err, "paged decoder step");
+  if (site != 0) {
+    e->last_error = "cruise_decoder_step_paged: a tensor-core GEMM wait gave up (site " + std::to_string(site) + ")";
+    return -3;
+  }
+  return 0;
+}
+
 int32_t synth_all(Engine *e, uint64_t seed, double stddev) {
   const ModelDims &m = e->m;
   const double sigma = 2.0 * std::sqrt(4.0 * (65536.0 * 65536.0 - 1.0) / 12.0);
@@ -1431,7 +1654,7 @@ int32_t run_decoder_step(Engine *e, const int64_t *token, const int64_t *positio
   err = cudaMemcpyAsync(&io->history, &e->d_io->history, sizeof(EpochIO) - offsetof(EpochIO, history),
                         cudaMemcpyDeviceToHost, e->stream);
   if (err == cudaSuccess)
-    err = cudaMemcpyAsync(logits_out, e->logits, sizeof(float) * kBatch * m.V, cudaMemcpyDeviceToHost, e->stream);
+    err = cudaMemcpyAsync(logits_out, e->logits, sizeof(float) * kBatch * m.V, cudaMemcpyDefault, e->stream);
   if (err == cudaSuccess) err = cudaStreamSynchronize(e->stream);
   if (err != cudaSuccess) return set_err(e, err, "decoder step completion");
   cudaEventElapsedTime(&e->last_ms, e->ev0, e->ev1);
@@ -1948,6 +2171,24 @@ int32_t cruise_decoder_step(void *engine, const int64_t *token, const int64_t *p
   std::lock_guard<std::mutex> lock(e->execute_mutex);
   return cruise::run_decoder_step(e, token, position, seq_len, key_cache, slot, active, block_table, value_cache,
                                   logits_out, next_position_out);
+}
+
+int32_t cruise_decoder_step_paged(void *engine, int32_t rows, const int64_t *token, const int64_t *position, void *key_cache,
+                                  void *value_cache, int64_t num_blocks, int32_t block_size, const int32_t *block_table,
+                                  int64_t table_stride, int32_t table_width, const void *rope_cos, const void *rope_sin,
+                                  int32_t rope_dtype, int32_t rope_rows, uint16_t *logits, int64_t logits_stride,
+                                  void *stream) {
+  if (engine == nullptr || token == nullptr || position == nullptr || key_cache == nullptr || value_cache == nullptr ||
+      block_table == nullptr || logits == nullptr)
+    return -1;
+  Engine *e = static_cast<Engine *>(engine);
+  std::lock_guard<std::mutex> lock(e->execute_mutex);
+  cudaSetDevice(e->device);
+  const cruise::PagedStep step{rows, token, position, static_cast<cruise::bf16 *>(key_cache),
+                               static_cast<cruise::bf16 *>(value_cache), num_blocks, block_size, block_table, table_stride,
+                               table_width, rope_cos, rope_sin, rope_dtype, rope_rows, logits, logits_stride,
+                               static_cast<cudaStream_t>(stream)};
+  return cruise::run_decoder_step_paged(e, step);
 }
 
 int32_t cruise_epoch_last_timing(void *engine, double *device_us, int32_t *kernel_launches) {

@@ -327,6 +327,39 @@ __global__ void qkv_rope_store(const float *acc, int nsplit, int T, const bf16 *
   }
 }
 
+// First kernel of a decoder step over caller-held paged caches, one CTA per
+// row: h = embed[token]; slot and length of the row's position.  A row whose
+// position is negative or past its table, or whose token does not exist, is
+// inactive: h is zero, nothing is stored (slot -1) and it attends to nothing.
+__global__ void paged_rows(const bf16 *embed, const int64_t *token, const int64_t *position, const int32_t *table,
+                           int64_t table_stride, int32_t table_width, int32_t block_size, int64_t num_blocks,
+                           int32_t rope_rows, int32_t vocab, bf16 *h, int32_t *slot, int32_t *length, int H) {
+  const int t = blockIdx.x;
+  const int64_t id = token[t], pos = position[t];
+  const bool active = id >= 0 && id < vocab && pos >= 0 && pos < rope_rows &&
+                      pos < static_cast<int64_t>(table_width) * block_size;
+  if (threadIdx.x == 0) {
+    const int64_t block = active ? table[t * table_stride + pos / block_size] : -1;
+    slot[t] = block >= 0 && block < num_blocks ? static_cast<int32_t>(block * block_size + pos % block_size) : -1;
+    length[t] = active ? static_cast<int32_t>(pos + 1) : 0;
+  }
+  const uint4 *src = reinterpret_cast<const uint4 *>(embed + (active ? id : 0) * static_cast<int64_t>(H));
+  uint4 *dst = reinterpret_cast<uint4 *>(h + static_cast<int64_t>(t) * H);
+  for (int i = threadIdx.x; i < H / 8; i += blockDim.x) dst[i] = active ? src[i] : make_uint4(0, 0, 0, 0);
+}
+
+// q, k, v = bf16(acc + bias) as rows [T][N] (F.linear: fp32 sum plus bias, one
+// rounding), two elements a thread.
+__global__ void qkv_bias_rows(const float *acc, int nsplit, int T, const bf16 *bias, bf16 *qkv, int N) {
+  chain_enter();
+  const int n = 2 * (blockIdx.y * blockDim.x + threadIdx.x), t = blockIdx.x;
+  if (n >= N) return;
+  const float2 s = split_sum2(acc, static_cast<int64_t>(T) * N, nsplit, static_cast<int64_t>(t) * N + n);
+  const __nv_bfloat162 b2 = *reinterpret_cast<const __nv_bfloat162 *>(bias + n);
+  *reinterpret_cast<uint32_t *>(qkv + static_cast<int64_t>(t) * N + n) =
+      bf2_bits(__fadd_rn(s.x, __low2float(b2)), __fadd_rn(s.y, __high2float(b2)));
+}
+
 // Tokens of the cohort in the order the host packs them: row by row, each
 // row's positions 0..count-1 consecutive from `start`.
 struct RowSpans {

@@ -221,13 +221,14 @@ class EpochEngine:
 
     # -- one decoder step (9-in / 4-out decoder ABI) ---------------------------------
     def decoder_step(self, token, position, seq_len, slot, active, block_table, key: torch.Tensor | None = None,
-                     value: torch.Tensor | None = None, logits_out: np.ndarray | None = None
-                     ) -> tuple[np.ndarray, np.ndarray]:
+                     value: torch.Tensor | None = None, logits_out: np.ndarray | torch.Tensor | None = None
+                     ) -> tuple[np.ndarray | torch.Tensor, np.ndarray]:
         """One decoder call, no controller (``cruise_decoder_step``): returns the
         f32 logits [4, V] and the next positions [4].  ``key`` / ``value`` are
         caller-held bf16 CUDA caches in the engine's layout (updated in place),
         or None for the engine's resident caches.  ``logits_out`` may be a
-        preallocated f32 [4, V] array (for example a view of pinned memory)."""
+        preallocated f32 [4, V] array (for example a view of pinned memory), or
+        a CUDA tensor on the engine's device, which then is what is returned."""
         cfg = self.config
         token = np.ascontiguousarray(np.asarray(token, dtype=np.int64).reshape(BATCH))
         position = np.ascontiguousarray(np.asarray(position, dtype=np.int64).reshape(BATCH))
@@ -237,8 +238,17 @@ class EpochEngine:
         block_table = np.ascontiguousarray(
             np.asarray(block_table, dtype=np.int32).reshape(BATCH * cfg.blocks_per_row))
         logits = np.empty((BATCH, cfg.vocab), dtype=np.float32) if logits_out is None else logits_out
-        if logits.shape != (BATCH, cfg.vocab) or logits.dtype != np.float32 or not logits.flags.c_contiguous:
+        if isinstance(logits, torch.Tensor):
+            if (not logits.is_cuda or logits.get_device() != self.device or logits.dtype != torch.float32
+                    or tuple(logits.shape) != (BATCH, cfg.vocab) or not logits.is_contiguous()):
+                raise ValueError(f"logits_out must be a contiguous float32 [{BATCH}, {cfg.vocab}] tensor on cuda:{self.device}")
+            # the engine's stream does not order after torch's: what the tensor is still used for must be done
+            torch.cuda.current_stream(self.device).synchronize()
+            logits_ptr = ctypes.cast(logits.data_ptr(), ctypes.POINTER(ctypes.c_float))
+        elif logits.shape != (BATCH, cfg.vocab) or logits.dtype != np.float32 or not logits.flags.c_contiguous:
             raise ValueError(f"logits_out must be a contiguous float32 [{BATCH}, {cfg.vocab}] array")
+        else:
+            logits_ptr = _ptr(logits, ctypes.c_float)
         next_position = np.empty(BATCH, dtype=np.int64)
         caches = []
         for cache in (key, value):
@@ -252,10 +262,65 @@ class EpochEngine:
         rc = self.lib.cruise_decoder_step(
             self.handle, _ptr(token, ctypes.c_int64), _ptr(position, ctypes.c_int64), _ptr(seq_len, ctypes.c_int32),
             caches[0], _ptr(slot, ctypes.c_int32), _ptr(active, ctypes.c_int32), _ptr(block_table, ctypes.c_int32),
-            caches[1], None, _ptr(logits, ctypes.c_float), _ptr(next_position, ctypes.c_int64),
+            caches[1], None, logits_ptr, _ptr(next_position, ctypes.c_int64),
         )
         self._check(rc, "cruise_decoder_step")
         return logits, next_position
+
+    def decoder_step_paged(self, token: torch.Tensor, position: torch.Tensor, block_table: torch.Tensor,
+                           key: torch.Tensor, value: torch.Tensor, cos: torch.Tensor | None = None,
+                           sin: torch.Tensor | None = None, logits_out: torch.Tensor | None = None) -> torch.Tensor:
+        """One decoder step of any number of rows over caller-held paged caches of
+        any length (``cruise_decoder_step_paged``): the engine's projections
+        around :func:`cruise_b200.decoder_ops.rotate_store` and
+        :func:`cruise_b200.decoder_ops.paged_attention`.  CUDA tensors on the
+        engine's device: ``token`` and ``position`` int64 [rows] (a negative
+        position: the row is inactive), ``block_table`` int32 [rows, width],
+        ``key`` / ``value`` bf16 [layers, blocks, block_size, kv heads, head_dim]
+        (updated in place), ``cos`` / ``sin`` [positions, head_dim] bf16 or fp32
+        (the engine's tables by default).  Returns the logits bf16 [rows, V]
+        (``logits_out``); :func:`cruise_b200.decoder_ops.choose` takes them."""
+        cfg = self.config
+        tensors = dict(token=token, position=position, block_table=block_table, key=key, value=value, cos=cos, sin=sin,
+                       logits_out=logits_out)
+        for name, tensor in tensors.items():
+            if tensor is not None and (not isinstance(tensor, torch.Tensor) or not tensor.is_cuda
+                                       or tensor.get_device() != self.device):
+                raise ValueError(f"{name} must be a tensor on cuda:{self.device}")
+        rows = token.shape[0]
+        for name in ("token", "position"):
+            if tensors[name].dtype != torch.int64 or tuple(tensors[name].shape) != (rows,) or not tensors[name].is_contiguous():
+                raise ValueError(f"{name} must be contiguous int64 [{rows}]")
+        if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != rows
+                or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
+            raise ValueError(f"block_table must be int32 [{rows}, width] with contiguous rows")
+        heads = (self.shard.nkv, cfg.head_dim)
+        for name in ("key", "value"):
+            cache = tensors[name]
+            if (cache.dtype != torch.bfloat16 or cache.dim() != 5 or cache.shape[0] != cfg.num_layers
+                    or tuple(cache.shape[3:]) != heads or cache.shape != key.shape or not cache.is_contiguous()):
+                raise ValueError(f"{name} must be contiguous bf16 [{cfg.num_layers}, blocks, block_size, {heads[0]}, {heads[1]}]")
+        if (cos is None) != (sin is None):
+            raise ValueError("pass both rotation tables or neither")
+        codes = {torch.bfloat16: 0, torch.float32: 2}
+        if cos is not None and (cos.dim() != 2 or cos.shape[1] != cfg.head_dim or cos.shape != sin.shape or cos.dtype not in codes
+                                or sin.dtype != cos.dtype or not cos.is_contiguous() or not sin.is_contiguous()):
+            raise ValueError(f"cos and sin must be contiguous bf16 or fp32 [positions, {cfg.head_dim}]")
+        if logits_out is None:
+            logits_out = torch.empty((rows, cfg.vocab), dtype=torch.bfloat16, device=token.device)
+        if (logits_out.dtype != torch.bfloat16 or tuple(logits_out.shape) != (rows, cfg.vocab) or logits_out.stride(1) != 1):
+            raise ValueError(f"logits_out must be bf16 [{rows}, {cfg.vocab}] with contiguous rows")
+        if rows == 0:
+            return logits_out
+        rc = self.lib.cruise_decoder_step_paged(
+            self.handle, rows, token.data_ptr(), position.data_ptr(), key.data_ptr(), value.data_ptr(), key.shape[1],
+            key.shape[2], block_table.data_ptr(), block_table.stride(0) if rows > 1 else block_table.shape[1],
+            block_table.shape[1], None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(),
+            0 if cos is None else codes[cos.dtype], 0 if cos is None else cos.shape[0], logits_out.data_ptr(),
+            logits_out.stride(0) if rows > 1 else cfg.vocab, torch.cuda.current_stream(self.device).cuda_stream,
+        )
+        self._check(rc, "cruise_decoder_step_paged")
+        return logits_out
 
     # -- batched device prefill -------------------------------------------------------
     def prefill(self, prompts) -> None:

@@ -260,8 +260,9 @@ int32_t cruise_epoch_run_noalloc(void *engine, const int64_t *token,
  * [kv_heads][head_dim] on the engine's device, 16-byte aligned, updated in
  * place (the ABI's K and V outputs); both NULL for the engine's resident
  * caches.
- * Outputs (host): logits_out f32 [4][vocab], next_position_out i64[4] =
- * position + 1 for active rows, position otherwise.
+ * Outputs: logits_out f32 [4][vocab] (host memory, or device memory of the
+ * engine's device, ready when the call returns), next_position_out (host)
+ * i64[4] = position + 1 for active rows, position otherwise.
  * For active rows the step computes exactly what the reference decoder does
  * (batched_decoder_step.py:277-417): the new K/V are written at slot[row]
  * and attention covers positions < seq_len.  Rows with active 0 write no K/V
@@ -281,6 +282,33 @@ int32_t cruise_decoder_step(void *engine, const int64_t *token,
                             const int32_t *active, const int32_t *block_table,
                             void *value_cache, const uint8_t *tiling,
                             float *logits_out, int64_t *next_position_out);
+
+/* One decoder step of any number of rows over caller-held paged caches of any
+ * length, layer by layer: the engine's projections around the decoder
+ * operators of cruise_decoder.h (rotate_store and paged_attention), where the
+ * resident kernel holds four rows of blocks_per_row blocks.  Every array is
+ * device memory on the engine's device: token i64[rows] and position i64[rows]
+ * (negative: the row is inactive), caches bf16 [layers][num_blocks][block_size]
+ * [kv_heads][head_dim] (16-byte aligned, updated in place at each position's
+ * slot), block_table i32 [rows][table_width] (rows table_stride entries apart),
+ * rope_cos / rope_sin [rope_rows][head_dim] of rope_dtype 0 (bf16) or 2 (fp32),
+ * or both NULL for the engine's own tables.  A row whose token or position does
+ * not exist is inactive too; the logits of inactive rows must not be used.  Two
+ * rows must not share a slot.  rows at most 4 block_size of the engine.
+ * logits: bf16 [rows][vocab], rows logits_stride elements apart (the decoder's
+ * rounding: cruise_decoder_step gives the same values as f32).  Rounds where the
+ * decoder does, but for the attention's scores and probabilities and the
+ * rotation, which stay in fp32.
+ * Waits for what `stream` holds, and returns when the step has completed.
+ * Returns 0, -1 for invalid arguments, -2 when a projection could not be
+ * launched, -3 when a device-side wait gave up, -4 for a tensor-parallel
+ * engine, or a CUDA error code; cruise_epoch_last_error explains them. */
+int32_t cruise_decoder_step_paged(
+    void *engine, int32_t rows, const int64_t *token, const int64_t *position,
+    void *key_cache, void *value_cache, int64_t num_blocks, int32_t block_size,
+    const int32_t *block_table, int64_t table_stride, int32_t table_width,
+    const void *rope_cos, const void *rope_sin, int32_t rope_dtype,
+    int32_t rope_rows, uint16_t *logits, int64_t logits_stride, void *stream);
 
 /* Device time of the last epoch (or decoder step) in microseconds (CUDA
  * events around the epoch kernel) and the number of kernels it launched. */
