@@ -45,6 +45,7 @@ struct AttentionPlan {
   int32_t units;       // units per row: nkv * chunks
   int32_t block_shift; // log2(block_size), -1 when not a power of two
   int32_t capacity;    // table_width * block_size
+  uint32_t block_chunks, slot_chunks;   // 16-byte chunks between blocks and between slots
   float scale_log2;    // scale * log2(e)
   float *piece_o;      // [2 grid][heads][d]
   float *piece_ml;     // [2 grid][heads][2]
@@ -114,16 +115,14 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
   const AttentionArgs &a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, q2 = (lane & 3) * 2;
-  if constexpr (!Whole) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  follow_predecessor();
 
   // -- this CTA's share of the work (row-major, units of a row; a unit is its
   // set-up, then its tiles) --
   constexpr int kSetup = attend_setup(D);
-  int row, off, left;
+  int row, off = 0, left = 1;
   if constexpr (Whole) {
     row = blockIdx.x / p.units;
-    left = row_tiles<Warps>(row_length(p, row)) + kSetup;
-    off = (blockIdx.x - row * p.units) * left;
   } else {
     const int per = (a.rows + kAttendThreads - 1) / kAttendThreads;
     const int r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
@@ -176,24 +175,43 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
   const uint32_t ring_addr = smem_u32(my_ring);
 
   while (left > 0) {
-    const int length = row_length(p, row);
-    const int n = row_tiles<Warps>(length), cost = n + kSetup;
-    const int unit = off / cost, at0 = off - unit * cost;
-    const int take = min(cost - at0, left);
-    const int t0 = max(0, at0 - kSetup), count = max(0, at0 + take - kSetup) - t0;
-    off += take;
-    left -= take;
-    const int row_now = row;
-    if (off == cost * p.units) {
-      off = 0;
-      ++row;
+    const int length = row_length(p, row), row_now = row;
+    const int n = row_tiles<Warps>(length);
+    int unit, t0, count;
+    if constexpr (Whole) {
+      unit = blockIdx.x - row * p.units;   // (known before the length)
+      t0 = 0;
+      count = n;
+      left = 0;
+    } else {
+      const int cost = n + kSetup;
+      unit = off / cost;
+      const int at0 = off - unit * cost, take = min(cost - at0, left);
+      t0 = max(0, at0 - kSetup);
+      count = max(0, at0 + take - kSetup) - t0;
+      off += take;
+      left -= take;
+      if (off == cost * p.units) {
+        off = 0;
+        ++row;
+      }
+      if (count == 0) continue;   // only the set-up of a unit that the next CTA takes
     }
-    if (count == 0) continue;   // only the set-up of a unit that the next CTA takes
     const int kvh = unit / p.chunks, head0 = kvh * p.groups + (unit - kvh * p.chunks) * p.chunk;
     const int heads = min(p.chunk, (kvh + 1) * p.groups - head0);
     const int32_t *table = a.block_table + row_now * a.table_stride;
     const T *kbase = static_cast<const T *>(a.key_cache) + kvh * D;
     const T *vbase = static_cast<const T *>(a.value_cache) + kvh * D;
+
+    // the block of this lane's key of step i, fetched a step before its use (the
+    // copies of a step do not wait for the table) and without the row's length
+    // (the first step waits for one load, not two)
+    auto block_of = [&](int i) {
+      const int t = (t0 + i) * kAttendTile + warp * kAttendKeys + lane;
+      if (lane >= kAttendKeys || t >= p.capacity) return -1;
+      return table[p.block_shift >= 0 ? t >> p.block_shift : t / a.block_size];
+    };
+    int next_block = block_of(0);
 
     // Q fragments: column n of the product is head head0 + 8 nt + n
     uint32_t qf[NT][D / 16][2];
@@ -208,36 +226,32 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
       }
     }
 
-    // the block of this lane's key of step i (-1: none), fetched a step before
-    // its use: the copies of a step do not wait for the table
-    auto block_of = [&](int i) {
-      const int t = (t0 + i) * kAttendTile + warp * kAttendKeys + lane;
-      if (i >= count || lane >= kAttendKeys || t >= length) return -1;
-      return table[p.block_shift >= 0 ? t >> p.block_shift : t / a.block_size];
-    };
-    int next_block = block_of(0);
     auto load = [&](int i, int stage) {
       const int id = next_block;
       next_block = block_of(i + 1);
       const int t = (t0 + i) * kAttendTile + warp * kAttendKeys + lane;
-      const bool live = id >= 0 && id < a.num_blocks;
-      int64_t at = 0;
+      const bool live = i < count && t < length && id >= 0 && id < a.num_blocks;
+      uint32_t at = 0;   // the key's row, in 16-byte chunks of the cache
       if (live) {
         const int in = p.block_shift >= 0 ? t & (a.block_size - 1) : t % a.block_size;
-        at = id * a.block_stride + static_cast<int64_t>(in) * a.nkv * D;
+        at = static_cast<uint32_t>(id) * p.block_chunks + static_cast<uint32_t>(in) * p.slot_chunks;
       }
       const uint32_t mask = __ballot_sync(0xffffffffu, live);
       if (lane == 0) live_mask[warp][stage] = mask;
-      const uint32_t kdst = ring_addr + stage * S::kStageBytes, vdst = kdst + kAttendKeys * S::kRowBytes;
-      if (i < count) {
+      if (mask != 0) {
+        // lane l copies chunk l % kChunks of the keys kKeys j + l / kChunks; a row's
+        // chunks lie permuted by chunk ^ (key & 7) against bank conflicts
+        constexpr int kKeys = 32 / kChunks;
+        const int c = lane % kChunks, k0 = lane / kChunks;
+        const uint32_t kdst = ring_addr + stage * S::kStageBytes + k0 * S::kRowBytes, swizzle = (c ^ k0) << 4;
+        const uint4 *const ksrc = reinterpret_cast<const uint4 *>(kbase) + c, *const vsrc = reinterpret_cast<const uint4 *>(vbase) + c;
 #pragma unroll
-        for (int j = 0; j < kAttendKeys * kChunks / 32; ++j) {
-          const int idx = j * 32 + lane, key = idx / kChunks, c = idx % kChunks;
-          const int64_t src = __shfl_sync(0xffffffffu, at, key) + c * 8;
-          const int bytes = (mask >> key) & 1 ? 16 : 0;
-          const uint32_t dst = key * S::kRowBytes + ((c ^ (key & 7)) << 4);
-          cp_async16_zfill(kdst + dst, kbase + src, bytes);
-          cp_async16_zfill(vdst + dst, vbase + src, bytes);
+        for (int j = 0; j < kAttendKeys / kKeys; ++j) {
+          const uint32_t from = __shfl_sync(0xffffffffu, at, j * kKeys + k0);
+          const int bytes = (mask >> (j * kKeys + k0)) & 1 ? 16 : 0;
+          const uint32_t dst = kdst + j * kKeys * S::kRowBytes + (swizzle ^ (((j * kKeys) & 7) << 4));
+          cp_async16_zfill(dst, ksrc + from, bytes);
+          cp_async16_zfill(dst + kAttendKeys * S::kRowBytes, vsrc + from, bytes);
         }
       }
       cp_async_commit();
@@ -342,25 +356,28 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
     __syncthreads();   // every warp is done with its ring
     const bool whole = t0 == 0 && count == n;
     const int64_t piece = 2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0);
-    if (tid < heads) {   // the head's maximum and sum, each warp's factor, lse
-      float top = -INFINITY, sum = 0.f;
+    if (tid < (heads * Warps + 31) / 32 * 32) {   // whole warps: a lane per (head, warp)
+      // the head's maximum and sum over the warps, each warp's factor, lse
+      const int h = tid / Warps, w = tid % Warps;
+      const bool live = h < heads;
+      const float m_w = live ? merge_ml[w][h][0] : -INFINITY, l_w = live ? merge_ml[w][h][1] : 0.f;
+      float top = m_w;
 #pragma unroll
-      for (int w = 0; w < Warps; ++w) top = fmaxf(top, merge_ml[w][tid][0]);
-      const float base = top == -INFINITY ? 0.f : top;
-      float f[Warps];
+      for (int o = 1; o < Warps; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float f = exp2f(m_w - (top == -INFINITY ? 0.f : top));
+      float sum = l_w * f;
 #pragma unroll
-      for (int w = 0; w < Warps; ++w) {
-        f[w] = exp2f(merge_ml[w][tid][0] - base);
-        sum = fmaf(merge_ml[w][tid][1], f[w], sum);
-      }
-      // a whole unit is divided here; no key with a weight gives zeros and log 0
-      const float scale = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-      for (int w = 0; w < Warps; ++w) merge_f[w][tid] = f[w] * scale;
-      if (!whole) {
-        *reinterpret_cast<float2 *>(p.piece_ml + (piece * (NT * 8) + tid) * 2) = make_float2(top, sum);
-      } else if (a.lse != nullptr) {
-        a.lse[static_cast<int64_t>(row_now) * a.nq + head0 + tid] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+      for (int o = 1; o < Warps; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (live) {
+        // a whole unit is divided here; no key with a weight gives zeros and log 0
+        merge_f[w][h] = !whole ? f : sum == 0.f ? 0.f : f / sum;
+        if (w == 0) {
+          if (!whole) {
+            *reinterpret_cast<float2 *>(p.piece_ml + (piece * (NT * 8) + h) * 2) = make_float2(top, sum);
+          } else if (a.lse != nullptr) {
+            a.lse[static_cast<int64_t>(row_now) * a.nq + head0 + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+          }
+        }
       }
     }
 #pragma unroll
@@ -415,7 +432,7 @@ __global__ void __launch_bounds__(kJoinThreads, 1) attention_join_kernel(const A
   constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
   __shared__ __align__(16) float red[kGroups][D];
   __shared__ float red_ml[kGroups][2];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  follow_predecessor();
   const int4 of = p.piece_of[blockIdx.x];
   const int pieces = of.z;
   if (pieces == 0) return;

@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
   const int tid = threadIdx.x, row = blockIdx.y, ctas = gridDim.x;
   const int part = ctas > 1 ? static_cast<int>(cluster_rank()) : 0;
   if (ctas > 1) cluster_arrive();   // every CTA of the cluster runs before its shared memory is written
+  wait_predecessor();
   const int32_t v0 = min(part * slice, a.vocab);
   const int32_t width = min(slice, a.vocab - v0);
   const T *const logits = static_cast<const T *>(a.logits) + row * a.logits_stride + v0;
@@ -209,6 +210,7 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
           if (i0 != tid) fetch(id, i0, counted);
 #pragma unroll
           for (int k = 0; k < kChooseBatch; ++k) {
+            if (i0 - tid + k * kChooseTableThreads >= counted) break;   // uniform: short histories run little code
             const int32_t i = i0 + k * kChooseTableThreads;
             const uint32_t n = here(id[k]);
             if (i < counted && n < static_cast<uint32_t>(width)) f(i, n);
@@ -289,16 +291,14 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
       constexpr int kTogether = 4;
       for (int32_t i0 = tid; i0 < listed; i0 += kTogether * kChooseTableThreads) {
         T raw[kTogether];
-        uint32_t n[kTogether];
 #pragma unroll
-        for (int k = 0; k < kTogether; ++k) {
-          n[k] = list[min(i0 + k * kChooseTableThreads, listed - 1)];
-          raw[k] = logits[n[k]];
-        }
-#pragma unroll
-        for (int k = 0; k < kTogether; ++k) {
+        for (int k = 0; k < kTogether; ++k) raw[k] = logits[list[min(i0 + k * kChooseTableThreads, listed - 1)]];
+#pragma unroll 1
+        for (int k = 0; k < kTogether && i0 - tid + k * kChooseTableThreads < listed; ++k) {
           const int32_t i = i0 + k * kChooseTableThreads;
-          if (i < listed && (counts[i] & kHasBias) == 0) rules(n[k], i, Logit<T>::one(&raw[k]));
+          if (i < listed && (counts[i] & kHasBias) == 0) rules(list[i], i, Logit<T>::one(&raw[0]));
+#pragma unroll
+          for (int q = 0; q + 1 < kTogether; ++q) raw[q] = raw[q + 1];
         }
       }
       if (biases > 0) named_sync(1, kChooseTableThreads);
@@ -409,6 +409,9 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
         }
       }
     };
+    // only now: a successor's CTAs that came earlier would take the SMs that this
+    // launch left idle two at a time, and run at half their pace later
+    release_successor();
     const bool retake = top_at >= 0 && ruled(top_at);
     if (retake) {
       top = -INFINITY;

@@ -68,19 +68,26 @@ cudaError_t allow_shared(Kernel kernel, size_t bytes, int device, std::atomic<ui
   return err;
 }
 
-// A kernel that joins what the one before it in the stream leaves: it may start
-// while that one drains and waits for it inside (griddepcontrol.wait).
+// Launches a kernel so that it may come onto the SMs while its predecessor in
+// the stream drains; it waits for that inside (follow_predecessor).  `cluster`
+// CTAs of x share their shared memory.
 template <typename... Params, typename... Actual>
-cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, const Actual &...args) {
+cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, size_t shared, int cluster, cudaStream_t stream,
+                   const Actual &...args) {
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = shared;
   cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -97,11 +104,8 @@ cudaError_t rotate_typed(const RotateArgs &a, int device, cudaStream_t stream) {
   const int warps_per_token = (all + rounds - 1) / rounds;
   const int64_t warps = static_cast<int64_t>(a.tokens) * warps_per_token;
   const unsigned grid = static_cast<unsigned>((warps * 32 + kRotateThreads - 1) / kRotateThreads);
-  if (a.q_norm != nullptr)
-    rotate_store_kernel<T, D, true><<<grid, kRotateThreads, 0, stream>>>(a, rounds, warps_per_token);
-  else
-    rotate_store_kernel<T, D, false><<<grid, kRotateThreads, 0, stream>>>(a, rounds, warps_per_token);
-  return cudaGetLastError();
+  return launch(a.q_norm != nullptr ? rotate_store_kernel<T, D, true> : rotate_store_kernel<T, D, false>, dim3(grid),
+                kRotateThreads, 0, 1, stream, a, rounds, warps_per_token);
 }
 
 // ---- paged_attention -----------------------------------------------------------
@@ -149,6 +153,8 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
   for (int b = 0; b < 31; ++b)
     if (a.block_size == 1 << b) p.block_shift = b;
   p.capacity = a.table_width * a.block_size;
+  p.block_chunks = static_cast<uint32_t>(a.block_stride / 8);
+  p.slot_chunks = static_cast<uint32_t>(a.nkv * D / 8);
   p.scale_log2 = a.scale * 1.4426950408889634f;
   static std::atomic<uint64_t> done{0}, done_whole{0};
   if (s.whole) {
@@ -156,8 +162,7 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
     auto *kernel = attention_kernel<T, D, NT, kAttendWholeWarps, true>;
     const cudaError_t err = allow_shared(kernel, smem, device, done_whole);
     if (err != cudaSuccess) return err;
-    kernel<<<static_cast<unsigned>(a.rows) * s.units, kAttendWholeWarps * 32, smem, stream>>>(p);
-    return cudaGetLastError();
+    return launch(kernel, dim3(static_cast<unsigned>(a.rows) * s.units), kAttendWholeWarps * 32, smem, 1, stream, p);
   }
   p.by_unit = static_cast<int64_t>(a.rows) * s.units <= s.grid ? 1 : 0;
   size_t ml = 0, of = 0;
@@ -170,14 +175,13 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
   auto *kernel = attention_kernel<T, D, NT, kAttendWarps, false>;
   cudaError_t err = allow_shared(kernel, smem, device, done);
   if (err != cudaSuccess) return err;
-  kernel<<<s.grid, kAttendWarps * 32, smem, stream>>>(p);
-  err = cudaGetLastError();
+  err = launch(kernel, dim3(s.grid), kAttendWarps * 32, smem, 1, stream, p);
   if (err != cudaSuccess) return err;
   // few units: a CTA for some heads of each, so that the join is spread over the SMs
   const int64_t units = static_cast<int64_t>(a.rows) * s.units;
   const int entries = p.by_unit ? static_cast<int>(units) : s.grid;
   const int each = std::clamp((s.chunk * entries + sm_count(device) - 1) / sm_count(device), 1, s.chunk);
-  return launch_dependent(attention_join_kernel<T, D, NT>, dim3(entries, (s.chunk + each - 1) / each), kJoinThreads, stream, p, each);
+  return launch(attention_join_kernel<T, D, NT>, dim3(entries, (s.chunk + each - 1) / each), kJoinThreads, 0, 1, stream, p, each);
 }
 
 template <typename T>
@@ -204,19 +208,7 @@ cudaError_t choose_typed(const ChooseArgs &a, int device, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
   cudaError_t err = allow_shared(choose_kernel<T>, kChooseShared, device, done, true);
   if (err != cudaSuccess) return err;
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(ctas);
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.gridDim = dim3(ctas, a.rows);
-  cfg.blockDim = dim3(kChooseThreads);
-  cfg.dynamicSmemBytes = choose_shared(slice, entries);
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, choose_kernel<T>, a, slice);
+  return launch(choose_kernel<T>, dim3(ctas, a.rows), kChooseThreads, choose_shared(slice, entries), ctas, stream, a, slice);
 }
 
 // ---- errors --------------------------------------------------------------------
@@ -381,6 +373,9 @@ int32_t cruise_decoder_attention(const void *q, int64_t q_stride, int32_t rows, 
                   static_cast<long long>(table_stride));
   if (q_stride % 8 != 0 || out_stride % 8 != 0 || block_stride % 8 != 0)
     return refuse("%s: strides must be multiples of 8 elements", op);
+  if (num_blocks > (int64_t(1) << 35) / block_stride)
+    return refuse("%s: %lld blocks %lld elements apart pass 2^35 elements", op, static_cast<long long>(num_blocks),
+                  static_cast<long long>(block_stride));
   if (!(scale - scale == 0.f)) return refuse("%s: the scale must be finite", op);
   if (rows == 0) return report(cudaSuccess, op);
   if (q == nullptr || key_cache == nullptr || value_cache == nullptr || seq_len == nullptr || out == nullptr ||

@@ -74,6 +74,7 @@ template <typename T, int D, bool Norm>
 __global__ void __launch_bounds__(kRotateThreads, kRotateCtas) rotate_store_kernel(const RotateArgs a, int rounds, int warps_per_token) {
   constexpr int kLanes = D / 16;
   constexpr int kHeads = 32 / kLanes;
+  follow_predecessor();
   const int64_t warp = (static_cast<int64_t>(blockIdx.x) * kRotateThreads + threadIdx.x) >> 5;
   const int64_t t = warp / warps_per_token;
   if (t >= a.tokens) return;   // uniform over the warp

@@ -1242,6 +1242,8 @@ int32_t run_decoder_step_paged(Engine *e, const PagedStep &s) {
     return reject("caches and tables need at least one block, below 2^31 slots and 2^30 positions a row");
   if (static_cast<int64_t>(s.rows) * m.nkv * ((m.nq / m.nkv + 15) / 16) * (capacity / 64 + 8) > 0x7fffffff)
     return reject("rows x KV heads x capacity / 64 passes 2^31");
+  if (s.num_blocks > (int64_t(1) << 35) / (static_cast<int64_t>(s.block_size) * m.nkv * m.d))
+    return reject("a layer's cache passes 2^35 elements");
   if (s.logits_stride < m.V) return reject("the stride of the logits is smaller than the vocabulary");
   if ((s.rope_cos == nullptr) != (s.rope_sin == nullptr)) return reject("pass both rotation tables or neither");
   if (s.rope_cos != nullptr && ((s.rope_dtype != ops::kBf16 && s.rope_dtype != ops::kFp32) || s.rope_rows < 1))

@@ -58,12 +58,12 @@ int32_t cruise_decoder_rotate_store(
  * apart) = softmax(scale q K^T) V, lse (may be NULL) [rows][num_heads] fp32 the
  * natural logarithm of the softmax's sum.  Positions whose block lies outside
  * [0, num_blocks) are left out; a row with no position left gets zeros and
- * lse -inf.  Table entries past a row's length are not read.
+ * lse -inf.  The values of table entries past a row's length do not matter.
  * workspace: cruise_decoder_attention_workspace() bytes, 16-byte aligned, not
  * shared by calls that may overlap (its contents do not matter between calls);
  * NULL where that returns 0.  Other pointers 16-byte aligned (block_table,
  * seq_len, lse 4-byte), strides of q, out and blocks multiples of 8 elements;
- * out must not overlap the inputs. */
+ * out must not overlap the inputs; num_blocks block_stride at most 2^35. */
 int32_t cruise_decoder_attention(
     const void *q, int64_t q_stride, int32_t rows, int32_t num_heads,
     int32_t num_kv_heads, int32_t head_dim, int32_t dtype,

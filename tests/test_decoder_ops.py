@@ -57,7 +57,7 @@ def test_rotate_store_refuses(change, reason):
     (dict(table_width=1 << 28, table_stride=1 << 28), "capacity"),
     (dict(rows=1 << 20, table_width=1 << 20, table_stride=1 << 20), "passes 2^31"),
     (dict(table_stride=1), "stride"), (dict(q_stride=252), "stride"), (dict(out_stride=260), "multiples of 8"),
-    (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(out=None), "NULL"),
+    (dict(num_blocks=1 << 20, block_stride=1 << 16), "2^35"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(out=None), "NULL"),
     (dict(block_table=None), "NULL"), (dict(q=at(0) + 2), "aligned"), (dict(out=at(0)), "overlap"),
     (dict(out=at(2) + 4096), "overlap"), (dict(lse=at(5) + 16), "overlap"), (dict(lse=at(4)), "overlap"),
     (dict(table_width=64, table_stride=64), "workspace"),
