@@ -38,6 +38,7 @@ constexpr int kChooseMaxCluster = 16;
 constexpr int kChooseAhead = 4;            // vectors a thread has in flight
 constexpr int kChooseBatch = 8;            // history entries a thread has in flight
 constexpr size_t kChooseShared = 200 * 1024;
+constexpr size_t kChooseAlone = 118 * 1024;   // shared memory that leaves an SM no second CTA
 constexpr int32_t kChooseMaxVocab = 1 << 20;
 constexpr uint32_t kInPrompt = 0x80000000u, kHasBias = 0x40000000u, kCount = 0x3fffffffu;
 
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
   const int tid = threadIdx.x, row = blockIdx.y, ctas = gridDim.x;
   const int part = ctas > 1 ? static_cast<int>(cluster_rank()) : 0;
   if (ctas > 1) cluster_arrive();   // every CTA of the cluster runs before its shared memory is written
-  wait_predecessor();
+  follow_predecessor();
   const int32_t v0 = min(part * slice, a.vocab);
   const int32_t width = min(slice, a.vocab - v0);
   const T *const logits = static_cast<const T *>(a.logits) + row * a.logits_stride + v0;
@@ -173,19 +174,23 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
   if (tid == 0) retakes = 0;
 
   if (active && tid < kChooseTableThreads) {
-    // -- the marked tokens; the first history entries are fetched with the lengths
-    // that say which of them count --
+    // -- the marked tokens.  What a thread does for an entry it does without
+    // branches (an entry of another slice marks nothing and counts nothing), so
+    // that a batch's entries overlap; the first history entries are fetched with
+    // the lengths that say which of them count --
     const int32_t *const history = a.history != nullptr ? a.history + row * a.history_stride : nullptr;
     const int32_t history_width = history != nullptr ? a.history_width : 0;
-    int32_t first_id[kChooseBatch];
-    auto fetch = [&](int32_t (&id)[kChooseBatch], int32_t i0, int32_t end) {
+    const bool has_bias = bias_token != nullptr && tid < a.bias_width;
+    int32_t id[kChooseBatch];
+    auto fetch = [&](int32_t i0, int32_t end) {
 #pragma unroll
       for (int k = 0; k < kChooseBatch; ++k) {
         const int32_t i = i0 + k * kChooseTableThreads;
         id[k] = i < end ? history[i] : -1;
       }
     };
-    fetch(first_id, tid, history_width);
+    fetch(tid, history_width);
+    const int32_t bias_id = has_bias ? bias_token[tid] : -1;
     int32_t length = 0, prompt = 0, biases = 0;
     float rep = 1.f, freq = 0.f, pres = 0.f;
     if (history != nullptr) {
@@ -197,36 +202,30 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
     if (a.frequency != nullptr) freq = a.frequency[row];
     if (a.presence != nullptr) pres = a.presence[row];
     const int32_t counted = rep != 1.f || freq != 0.f || pres != 0.f ? min(max(length, 0), history_width) : 0;
+    constexpr int32_t kStride = kChooseBatch * kChooseTableThreads;
     int32_t listed = 0;
     if (counted + biases > 0) {
       // a vocabulary id as a token of this slice; others are at least `width`
-      auto here = [&](int32_t id) { return static_cast<uint32_t>(id) - static_cast<uint32_t>(v0); };
-      // f(entry, token) for the slice's entries of the history
-      auto each = [&](auto &&f) {
-        int32_t id[kChooseBatch];
-#pragma unroll
-        for (int k = 0; k < kChooseBatch; ++k) id[k] = first_id[k];
-        for (int32_t i0 = tid; i0 < counted; i0 += kChooseBatch * kChooseTableThreads) {
-          if (i0 != tid) fetch(id, i0, counted);
-#pragma unroll
-          for (int k = 0; k < kChooseBatch; ++k) {
-            if (i0 - tid + k * kChooseTableThreads >= counted) break;   // uniform: short histories run little code
-            const int32_t i = i0 + k * kChooseTableThreads;
-            const uint32_t n = here(id[k]);
-            if (i < counted && n < static_cast<uint32_t>(width)) f(i, n);
-          }
-        }
-      };
+      auto here = [&](int32_t v) { return static_cast<uint32_t>(v) - static_cast<uint32_t>(v0); };
+      auto mark = [&](uint32_t n) { atomicOr(&marks[n >> 5], 1u << (n & 31)); };
       auto rank = [&](uint32_t n) { return ranks[n >> 5] + __popc(marks[n >> 5] & ((1u << (n & 31)) - 1)); };
       for (int32_t i = tid; i < words / 4; i += kChooseTableThreads) reinterpret_cast<uint4 *>(marks)[i] = make_uint4(0, 0, 0, 0);
       const int32_t most = min(counted + biases, width);
       for (int32_t i = tid; i < most; i += kChooseTableThreads) counts[i] = 0;
       named_sync(1, kChooseTableThreads);
-      each([&](int32_t, uint32_t n) { atomicOr(&marks[n >> 5], 1u << (n & 31)); });
-      for (int32_t i = tid; i < biases; i += kChooseTableThreads) {
-        const uint32_t n = here(bias_token[i]);
-        if (n < static_cast<uint32_t>(width)) atomicOr(&marks[n >> 5], 1u << (n & 31));
+      for (int32_t i0 = tid; i0 - tid < counted; i0 += kStride) {
+        if (i0 != tid) fetch(i0, counted);
+#pragma unroll
+        for (int k = 0; k < kChooseBatch; ++k) {
+          if (i0 - tid + k * kChooseTableThreads >= counted) break;   // uniform: short histories run little code
+          const uint32_t n = here(id[k]);
+          const bool mine = i0 + k * kChooseTableThreads < counted && n < static_cast<uint32_t>(width);
+          atomicOr(&marks[mine ? n >> 5 : 0], mine ? 1u << (n & 31) : 0u);
+        }
       }
+      if (here(bias_id) < static_cast<uint32_t>(width) && tid < biases) mark(here(bias_id));
+      for (int32_t i = tid + kChooseTableThreads; i < biases; i += kChooseTableThreads)
+        if (here(bias_token[i]) < static_cast<uint32_t>(width)) mark(here(bias_token[i]));
       named_sync(1, kChooseTableThreads);
       // ranks: every thread its run of words
       const int32_t per = (words / 4 + kChooseTableThreads - 1) / kChooseTableThreads * 4;
@@ -257,22 +256,28 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
         at = d + __popc(m.w);
       }
       named_sync(1, kChooseTableThreads);
-      each([&](int32_t i, uint32_t n) {
-        const uint32_t r = rank(n);
-        list[r] = n;   // the token's entries agree
-        if (i < prompt)
-          atomicOr(&counts[r], kInPrompt);
-        else
-          atomicAdd(&counts[r], 1u);
-      });
-      for (int32_t i = tid; i < biases; i += kChooseTableThreads) {
-        const uint32_t n = here(bias_token[i]);
+      for (int32_t i0 = tid; i0 - tid < counted; i0 += kStride) {
+        if (counted > kStride) fetch(i0, counted);
+#pragma unroll
+        for (int k = 0; k < kChooseBatch; ++k) {
+          if (i0 - tid + k * kChooseTableThreads >= counted) break;
+          const int32_t i = i0 + k * kChooseTableThreads;
+          const bool mine = i < counted && here(id[k]) < static_cast<uint32_t>(width);
+          const uint32_t n = mine ? here(id[k]) : 0, r = mine ? rank(n) : 0;   // (slot 0 exists)
+          if (mine) list[r] = n;   // the token's entries agree
+          atomicOr(&counts[r], mine && i < prompt ? kInPrompt : 0u);
+          atomicAdd(&counts[r], mine && i >= prompt ? 1u : 0u);
+        }
+      }
+      auto mark_bias = [&](uint32_t n) {
         if (n < static_cast<uint32_t>(width)) {
           const uint32_t r = rank(n);
           list[r] = n;
           atomicOr(&counts[r], kHasBias);
         }
-      }
+      };
+      if (tid < biases) mark_bias(here(bias_id));
+      for (int32_t i = tid + kChooseTableThreads; i < biases; i += kChooseTableThreads) mark_bias(here(bias_token[i]));
       named_sync(1, kChooseTableThreads);
       // the processed value takes the place of the occurrences
       auto rules = [&](uint32_t n, uint32_t r, float x) {
@@ -303,12 +308,12 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
       }
       if (biases > 0) named_sync(1, kChooseTableThreads);
       for (int32_t i = tid; i < biases; i += kChooseTableThreads) {   // entries of one token add up
-        const int32_t id = bias_token[i];
-        const uint32_t n = here(id);
-        if (n >= static_cast<uint32_t>(width) || (i > 0 && bias_token[i - 1] == id)) continue;
+        const int32_t v = bias_token[i];
+        const uint32_t n = here(v);
+        if (n >= static_cast<uint32_t>(width) || (i > 0 && bias_token[i - 1] == v)) continue;
         const float *const value = a.bias_value + row * a.bias_stride;
         float x = Logit<T>::one(logits + n);
-        for (int32_t j = i; j < biases && bias_token[j] == id; ++j) x = __fadd_rn(x, value[j]);
+        for (int32_t q = i; q < biases && bias_token[q] == v; ++q) x = __fadd_rn(x, value[q]);
         rules(n, rank(n), x);
       }
     }
@@ -409,9 +414,6 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
         }
       }
     };
-    // only now: a successor's CTAs that came earlier would take the SMs that this
-    // launch left idle two at a time, and run at half their pace later
-    release_successor();
     const bool retake = top_at >= 0 && ruled(top_at);
     if (retake) {
       top = -INFINITY;

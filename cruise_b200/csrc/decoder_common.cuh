@@ -15,11 +15,9 @@ namespace ops {
 // in the stream drains, lets its own successor do so, and waits for the
 // predecessor's completion (and its memory) before it reads or writes anything.
 // Calls one after the other then follow without a launch's latency between them.
-__device__ __forceinline__ void release_successor() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void follow_predecessor() {
-  release_successor();
-  wait_predecessor();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 template <typename T>

@@ -208,7 +208,12 @@ cudaError_t choose_typed(const ChooseArgs &a, int device, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
   cudaError_t err = allow_shared(choose_kernel<T>, kChooseShared, device, done, true);
   if (err != cudaSuccess) return err;
-  return launch(choose_kernel<T>, dim3(ctas, a.rows), kChooseThreads, choose_shared(slice, entries), ctas, stream, a, slice);
+  // Where every CTA can have an SM of its own it takes more than half its shared
+  // memory: a successor's CTAs, which come while this launch drains, would else
+  // settle two on the SMs it left idle (64 rows of 50257: 10.9 us, 9.4 so)
+  const size_t shared = choose_shared(slice, entries);
+  return launch(choose_kernel<T>, dim3(ctas, a.rows), kChooseThreads,
+                static_cast<int64_t>(a.rows) * ctas <= sms ? std::max(shared, kChooseAlone) : shared, ctas, stream, a, slice);
 }
 
 // ---- errors --------------------------------------------------------------------
