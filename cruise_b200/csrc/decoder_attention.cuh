@@ -61,6 +61,8 @@ struct AttendShared {
   static constexpr int kRowBytes = D * 2;
   static constexpr int kStageBytes = 2 * kAttendKeys * kRowBytes;   // K then V
   static constexpr int kRingBytes = Warps * kAttendStages * kStageBytes;
+  static constexpr int kMergeStride = D + 4;                        // fp32; no bank conflicts for the fragment stores
+  static constexpr int kMergeBytes = Warps * 8 * kMergeStride * 4;  // 8 heads of every warp
 };
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -105,12 +107,18 @@ template <typename T, int D, int NT, int Warps, bool Whole>
 __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attention_kernel(const AttentionPlan p) {
   using S = AttendShared<D, Warps>;
   constexpr int kAttendThreads = Warps * 32, kAttendTile = Warps * kAttendKeys;
+  // The ring, then the merge's room (a whole unit's CTA merges in the ring).  Two
+  // CTAs of head size 128 take the SM's shared memory to the last byte, so the
+  // few words beside them lie in the padding of the merge's rows.
   extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ uint32_t live_mask[Warps][kAttendStages];
   __shared__ float merge_ml[Warps][NT * 8][2];
-  __shared__ float merge_f[Warps][NT * 8];
-  __shared__ int scan[Warps];
-  __shared__ int found[3];
+  __shared__ float merge_f_room[NT == 1 ? Warps * 8 : 1];   // (16 heads: the factor replaces the maximum)
+  auto factor = [&](int w, int h) -> float & { return NT == 1 ? merge_f_room[w * 8 + h] : merge_ml[w][h][0]; };
+  uint32_t *const words = reinterpret_cast<uint32_t *>(ring + S::kRingBytes);
+  auto word = [&](int line, int i) -> uint32_t & {   // word i < 4 of 8 * Warps lines
+    return Whole ? words[line * 4 + i] : words[line * S::kMergeStride + D + i];
+  };
+  static_assert(kAttendStages <= 4, "a line holds a warp's masks");
   constexpr int kChunks = D / 8;   // 16-byte chunks of a row
   const AttentionArgs &a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -120,9 +128,10 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
   // -- this CTA's share of the work (row-major, units of a row; a unit is its
   // set-up, then its tiles) --
   constexpr int kSetup = attend_setup(D);
-  int row, off = 0, left = 1;
+  int row, off = 0, left = 1, length0;
   if constexpr (Whole) {
     row = blockIdx.x / p.units;
+    length0 = row_length(p, row);
   } else {
     const int per = (a.rows + kAttendThreads - 1) / kAttendThreads;
     const int r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
@@ -134,16 +143,16 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
       const int v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    if (lane == 31) scan[warp] = incl;
-    if (tid == 0) found[0] = -1;
+    if (lane == 31) word(Warps + warp, 0) = incl;
     __syncthreads();
     int total = 0;
     for (int w = 0; w < Warps; ++w) {
-      if (w < warp) incl += scan[w];
-      total += scan[w];
+      const int sum = static_cast<int>(word(Warps + w, 0));
+      if (w < warp) incl += sum;
+      total += sum;
     }
     total *= p.units;
-    const int share = max(2 * kSetup, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+    const int share = max(kSetup + 1, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
     const int64_t begin64 = static_cast<int64_t>(blockIdx.x) * share;
     if (begin64 >= total) {
       if (!p.by_unit && tid == 0) p.piece_of[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -155,63 +164,139 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
       for (int r = r0; r < r1; ++r) {
         const int n = row_tiles<Warps>(row_length(p, r)) + kSetup;
         if (begin < (before + n) * p.units) {
-          found[0] = r;
-          found[1] = begin - before * p.units;
-          found[2] = min(share, total - begin);
+          word(2 * Warps, 0) = r;
+          word(2 * Warps, 1) = begin - before * p.units;
+          word(2 * Warps, 2) = min(share, total - begin);
+          word(2 * Warps, 3) = row_length(p, r);
           break;
         }
         before += n;
       }
     }
     __syncthreads();
-    row = found[0];
-    off = found[1];
-    left = found[2];
+    row = word(2 * Warps, 0);
+    off = word(2 * Warps, 1);
+    left = word(2 * Warps, 2);
+    length0 = word(2 * Warps, 3);
   }
   const int share_work = left;   // the full share wherever a unit goes on after this CTA
   int4 tail = make_int4(0, 0, 0, 0);
 
+  // The CTA's work as segments, tiles of one unit each.  The copies run
+  // kAttendStages - 1 steps ahead of the products, over the segments' ends: the
+  // next unit's keys arrive while the last one's parts meet.
+  struct Segment {
+    int row, unit, n, t0, count, length;
+  };
+  struct Cursor {
+    int row, off, left, length, length_ahead;   // lengths of the row and the next
+  };
+  auto begin_at = [&]() {
+    Cursor c{row, off, left, length0, 0};
+    if (!Whole && row + 1 < a.rows) c.length_ahead = row_length(p, row + 1);
+    return c;
+  };
+  auto next_segment = [&](Cursor &c, Segment &s) {
+    while (c.left > 0) {
+      s.row = c.row;
+      s.length = c.length;
+      s.n = row_tiles<Warps>(s.length);
+      if constexpr (Whole) {
+        s.unit = blockIdx.x - c.row * p.units;   // (known before the length)
+        s.t0 = 0;
+        s.count = s.n;
+        c.left = 0;
+        return true;
+      } else {
+        const int cost = s.n + kSetup;
+        s.unit = c.off / cost;
+        const int at0 = c.off - s.unit * cost, take = min(cost - at0, c.left);
+        s.t0 = max(0, at0 - kSetup);
+        s.count = max(0, at0 + take - kSetup) - s.t0;
+        c.off += take;
+        c.left -= take;
+        if (c.off == cost * p.units) {
+          c.off = 0;
+          ++c.row;
+          c.length = c.length_ahead;
+          if (c.row + 1 < a.rows) c.length_ahead = row_length(p, c.row + 1);
+        }
+        if (s.count > 0) return true;   // else only the set-up of a unit that the next CTA takes
+      }
+    }
+    return false;
+  };
+
   uint8_t *const my_ring = ring + warp * kAttendStages * S::kStageBytes;
   const uint32_t ring_addr = smem_u32(my_ring);
-
-  while (left > 0) {
-    const int length = row_length(p, row), row_now = row;
-    const int n = row_tiles<Warps>(length);
-    int unit, t0, count;
-    if constexpr (Whole) {
-      unit = blockIdx.x - row * p.units;   // (known before the length)
-      t0 = 0;
-      count = n;
-      left = 0;
-    } else {
-      const int cost = n + kSetup;
-      unit = off / cost;
-      const int at0 = off - unit * cost, take = min(cost - at0, left);
-      t0 = max(0, at0 - kSetup);
-      count = max(0, at0 + take - kSetup) - t0;
-      off += take;
-      left -= take;
-      if (off == cost * p.units) {
-        off = 0;
-        ++row;
+  Cursor load_cursor = begin_at();
+  Segment from{};
+  int load_tile = 0, next_block = -1;
+  bool loading = true;
+  const int32_t *table = nullptr;
+  const uint4 *ksrc = nullptr, *vsrc = nullptr;
+  // the block of this lane's key of a tile, fetched a step before its use (the
+  // copies of a step do not wait for the table) and without the row's length
+  // (the first step waits for one load, not two)
+  auto block_of = [&](int i) {
+    const int t = (from.t0 + i) * kAttendTile + warp * kAttendKeys + lane;
+    if (lane >= kAttendKeys || t >= p.capacity) return -1;
+    return table[p.block_shift >= 0 ? t >> p.block_shift : t / a.block_size];
+  };
+  auto load = [&](int stage) {
+    if (loading && load_tile == from.count) {
+      loading = next_segment(load_cursor, from);
+      if (loading) {
+        const int kvh = from.unit / p.chunks;
+        table = a.block_table + from.row * a.table_stride;
+        ksrc = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.key_cache) + kvh * D) + lane % kChunks;
+        vsrc = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.value_cache) + kvh * D) + lane % kChunks;
+        load_tile = 0;
+        next_block = block_of(0);
       }
-      if (count == 0) continue;   // only the set-up of a unit that the next CTA takes
     }
+    uint32_t mask = 0;
+    if (loading) {
+      const int id = next_block;
+      next_block = block_of(load_tile + 1);
+      const int t = (from.t0 + load_tile) * kAttendTile + warp * kAttendKeys + lane;
+      const bool live = t < from.length && id >= 0 && id < a.num_blocks;
+      uint32_t at = 0;   // the key's row, in 16-byte chunks of the cache
+      if (live) {
+        const int in = p.block_shift >= 0 ? t & (a.block_size - 1) : t % a.block_size;
+        at = static_cast<uint32_t>(id) * p.block_chunks + static_cast<uint32_t>(in) * p.slot_chunks;
+      }
+      mask = __ballot_sync(0xffffffffu, live);
+      if (mask != 0) {
+        // lane l copies chunk l % kChunks of the keys kKeys j + l / kChunks; a row's
+        // chunks lie permuted by chunk ^ (key & 7) against bank conflicts
+        constexpr int kKeys = 32 / kChunks;
+        const int c = lane % kChunks, k0 = lane / kChunks;
+        const uint32_t kdst = ring_addr + stage * S::kStageBytes + k0 * S::kRowBytes, swizzle = (c ^ k0) << 4;
+#pragma unroll
+        for (int j = 0; j < kAttendKeys / kKeys; ++j) {
+          const uint32_t row_at = __shfl_sync(0xffffffffu, at, j * kKeys + k0);
+          const int bytes = (mask >> (j * kKeys + k0)) & 1 ? 16 : 0;
+          const uint32_t dst = kdst + j * kKeys * S::kRowBytes + (swizzle ^ (((j * kKeys) & 7) << 4));
+          cp_async16_zfill(dst, ksrc + row_at, bytes);
+          cp_async16_zfill(dst + kAttendKeys * S::kRowBytes, vsrc + row_at, bytes);
+        }
+      }
+      ++load_tile;
+    }
+    if (lane == 0) word(warp, stage) = mask;
+    cp_async_commit();
+  };
+
+  Cursor cursor = load_cursor;
+  Segment now{};
+#pragma unroll
+  for (int i = 0; i < kAttendStages - 1; ++i) load(i);
+  int stage = 0, fill = kAttendStages - 1;
+  while (next_segment(cursor, now)) {
+    const int unit = now.unit, t0 = now.t0, count = now.count, n = now.n, row_now = now.row;
     const int kvh = unit / p.chunks, head0 = kvh * p.groups + (unit - kvh * p.chunks) * p.chunk;
     const int heads = min(p.chunk, (kvh + 1) * p.groups - head0);
-    const int32_t *table = a.block_table + row_now * a.table_stride;
-    const T *kbase = static_cast<const T *>(a.key_cache) + kvh * D;
-    const T *vbase = static_cast<const T *>(a.value_cache) + kvh * D;
-
-    // the block of this lane's key of step i, fetched a step before its use (the
-    // copies of a step do not wait for the table) and without the row's length
-    // (the first step waits for one load, not two)
-    auto block_of = [&](int i) {
-      const int t = (t0 + i) * kAttendTile + warp * kAttendKeys + lane;
-      if (lane >= kAttendKeys || t >= p.capacity) return -1;
-      return table[p.block_shift >= 0 ? t >> p.block_shift : t / a.block_size];
-    };
-    int next_block = block_of(0);
 
     // Q fragments: column n of the product is head head0 + 8 nt + n
     uint32_t qf[NT][D / 16][2];
@@ -226,37 +311,6 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
       }
     }
 
-    auto load = [&](int i, int stage) {
-      const int id = next_block;
-      next_block = block_of(i + 1);
-      const int t = (t0 + i) * kAttendTile + warp * kAttendKeys + lane;
-      const bool live = i < count && t < length && id >= 0 && id < a.num_blocks;
-      uint32_t at = 0;   // the key's row, in 16-byte chunks of the cache
-      if (live) {
-        const int in = p.block_shift >= 0 ? t & (a.block_size - 1) : t % a.block_size;
-        at = static_cast<uint32_t>(id) * p.block_chunks + static_cast<uint32_t>(in) * p.slot_chunks;
-      }
-      const uint32_t mask = __ballot_sync(0xffffffffu, live);
-      if (lane == 0) live_mask[warp][stage] = mask;
-      if (mask != 0) {
-        // lane l copies chunk l % kChunks of the keys kKeys j + l / kChunks; a row's
-        // chunks lie permuted by chunk ^ (key & 7) against bank conflicts
-        constexpr int kKeys = 32 / kChunks;
-        const int c = lane % kChunks, k0 = lane / kChunks;
-        const uint32_t kdst = ring_addr + stage * S::kStageBytes + k0 * S::kRowBytes, swizzle = (c ^ k0) << 4;
-        const uint4 *const ksrc = reinterpret_cast<const uint4 *>(kbase) + c, *const vsrc = reinterpret_cast<const uint4 *>(vbase) + c;
-#pragma unroll
-        for (int j = 0; j < kAttendKeys / kKeys; ++j) {
-          const uint32_t from = __shfl_sync(0xffffffffu, at, j * kKeys + k0);
-          const int bytes = (mask >> (j * kKeys + k0)) & 1 ? 16 : 0;
-          const uint32_t dst = kdst + j * kKeys * S::kRowBytes + (swizzle ^ (((j * kKeys) & 7) << 4));
-          cp_async16_zfill(dst, ksrc + from, bytes);
-          cp_async16_zfill(dst + kAttendKeys * S::kRowBytes, vsrc + from, bytes);
-        }
-      }
-      cp_async_commit();
-    };
-
     float acc[NT][D / 16][4];
     float m[NT][2], l[NT][2];
 #pragma unroll
@@ -267,14 +321,11 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
       for (int dt = 0; dt < D / 16; ++dt) acc[nt][dt][0] = acc[nt][dt][1] = acc[nt][dt][2] = acc[nt][dt][3] = 0.f;
     }
 
-#pragma unroll
-    for (int i = 0; i < kAttendStages - 1; ++i) load(i, i);
-    int stage = 0, fill = kAttendStages - 1;
     for (int i = 0; i < count; ++i) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kAttendStages - 2) : "memory");
       __syncwarp();
-      const uint32_t mask = live_mask[warp][stage];
-      load(i + kAttendStages - 1, fill);   // the stage every lane left before the barrier above
+      const uint32_t mask = word(warp, stage);
+      load(fill);   // the stage every lane left before the barrier above
       if (mask != 0) {
         const uint32_t kaddr = ring_addr + stage * S::kStageBytes, vaddr = kaddr + kAttendKeys * S::kRowBytes;
         float s[NT][4], s2[NT][4];   // two chains: a product waits for the one before the last
@@ -336,11 +387,9 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
       stage = stage + 1 == kAttendStages ? 0 : stage + 1;
       fill = fill + 1 == kAttendStages ? 0 : fill + 1;
     }
-    cp_async_wait_all();
-
     // -- the warps' parts of the segment meet in shared memory --
-    constexpr int kStride = D + 4;   // fp32 row stride: no bank conflicts for the fragment stores
-    float *const merge = reinterpret_cast<float *>(ring);
+    if constexpr (Whole) cp_async_wait_all();   // the ring, done with, is the room for it
+    float *const merge = reinterpret_cast<float *>(Whole ? ring : ring + S::kRingBytes);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -353,7 +402,7 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
         }
       }
     }
-    __syncthreads();   // every warp is done with its ring
+    __syncthreads();   // every warp is done with its products, and with the merge before this one
     const bool whole = t0 == 0 && count == n;
     const int64_t piece = 2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0);
     if (tid < (heads * Warps + 31) / 32 * 32) {   // whole warps: a lane per (head, warp)
@@ -370,7 +419,7 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
       for (int o = 1; o < Warps; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (live) {
         // a whole unit is divided here; no key with a weight gives zeros and log 0
-        merge_f[w][h] = !whole ? f : sum == 0.f ? 0.f : f / sum;
+        factor(w, h) = !whole ? f : sum == 0.f ? 0.f : f / sum;
         if (w == 0) {
           if (!whole) {
             *reinterpret_cast<float2 *>(p.piece_ml + (piece * (NT * 8) + h) * 2) = make_float2(top, sum);
@@ -381,37 +430,38 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
       }
     }
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float *const h0 = merge + (warp * NT * 8 + nt * 8 + q2) * kStride + g;
+    for (int nt = 0; nt < NT; ++nt) {   // 8 heads at a time
+      if (nt > 0) __syncthreads();
+      float *const h0 = merge + (warp * 8 + q2) * S::kMergeStride + g;
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt) {
         h0[dt * 16] = acc[nt][dt][0];
-        h0[dt * 16 + kStride] = acc[nt][dt][1];
+        h0[dt * 16 + S::kMergeStride] = acc[nt][dt][1];
         h0[dt * 16 + 8] = acc[nt][dt][2];
-        h0[dt * 16 + 8 + kStride] = acc[nt][dt][3];
+        h0[dt * 16 + 8 + S::kMergeStride] = acc[nt][dt][3];
       }
-    }
-    __syncthreads();
-    for (int i = tid; i < heads * (D / 4); i += kAttendThreads) {   // four dimensions a thread
-      const int h = i / (D / 4), c = i % (D / 4) * 4;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      __syncthreads();
+      for (int i = tid; i < min(8, heads - nt * 8) * (D / 4); i += kAttendThreads) {   // four dimensions a thread
+        const int h = i / (D / 4), c = i % (D / 4) * 4;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < Warps; ++w) {
-        const float f = merge_f[w][h];
-        const float4 v = *reinterpret_cast<const float4 *>(merge + (w * NT * 8 + h) * kStride + c);
-        o.x = fmaf(v.x, f, o.x);
-        o.y = fmaf(v.y, f, o.y);
-        o.z = fmaf(v.z, f, o.z);
-        o.w = fmaf(v.w, f, o.w);
-      }
-      if (whole) {
-        *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + row_now * a.out_stride + static_cast<int64_t>(head0 + h) * D + c) =
-            make_uint2(Element<T>::pack(o.x, o.y), Element<T>::pack(o.z, o.w));
-      } else {
-        *reinterpret_cast<float4 *>(p.piece_o + piece * (NT * 8 * D) + h * D + c) = o;
+        for (int w = 0; w < Warps; ++w) {
+          const float f = factor(w, nt * 8 + h);
+          const float4 v = *reinterpret_cast<const float4 *>(merge + (w * 8 + h) * S::kMergeStride + c);
+          o.x = fmaf(v.x, f, o.x);
+          o.y = fmaf(v.y, f, o.y);
+          o.z = fmaf(v.z, f, o.z);
+          o.w = fmaf(v.w, f, o.w);
+        }
+        if (whole) {
+          *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + row_now * a.out_stride + static_cast<int64_t>(head0 + nt * 8 + h) * D + c) =
+              make_uint2(Element<T>::pack(o.x, o.y), Element<T>::pack(o.z, o.w));
+        } else {
+          *reinterpret_cast<float4 *>(p.piece_o + piece * (NT * 8 * D) + (nt * 8 + h) * D + c) = o;
+        }
       }
     }
-    __syncthreads();   // the ring is free for the next segment
+    if (NT > 1) __syncthreads();   // the factors have been read
     if (!Whole && t0 == 0) {
       const int4 of = make_int4(row_now, unit, whole ? 0 : 1 + (n - count + share_work - 1) / share_work, blockIdx.x);
       if (p.by_unit) {

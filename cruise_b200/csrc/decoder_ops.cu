@@ -104,8 +104,10 @@ cudaError_t rotate_typed(const RotateArgs &a, int device, cudaStream_t stream) {
   const int warps_per_token = (all + rounds - 1) / rounds;
   const int64_t warps = static_cast<int64_t>(a.tokens) * warps_per_token;
   const unsigned grid = static_cast<unsigned>((warps * 32 + kRotateThreads - 1) / kRotateThreads);
-  return launch(a.q_norm != nullptr ? rotate_store_kernel<T, D, true> : rotate_store_kernel<T, D, false>, dim3(grid),
-                kRotateThreads, 0, 1, stream, a, rounds, warps_per_token);
+  const bool full = a.rotary == D;
+  auto *kernel = a.q_norm != nullptr ? (full ? rotate_store_kernel<T, D, true, true> : rotate_store_kernel<T, D, true, false>)
+                                     : (full ? rotate_store_kernel<T, D, false, true> : rotate_store_kernel<T, D, false, false>);
+  return launch(kernel, dim3(grid), kRotateThreads, 0, 1, stream, a, rounds, warps_per_token);
 }
 
 // ---- paged_attention -----------------------------------------------------------
@@ -126,7 +128,7 @@ AttentionShape attention_shape(int32_t rows, int32_t nq, int32_t nkv, int32_t d,
   s.units = nkv * s.chunks;
   // few short rows: one CTA per unit and no second kernel
   const int sms = sm_count(device);
-  s.whole = capacity <= 4 * kAttendWholeWarps * kAttendKeys && static_cast<int64_t>(rows) * s.units <= sms;
+  s.whole = capacity <= 8 * kAttendWholeWarps * kAttendKeys && static_cast<int64_t>(rows) * s.units <= sms;
   s.grid = sms * attend_ctas(d);
   return s;
 }
@@ -158,7 +160,9 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
   p.scale_log2 = a.scale * 1.4426950408889634f;
   static std::atomic<uint64_t> done{0}, done_whole{0};
   if (s.whole) {
-    constexpr size_t smem = AttendShared<D, kAttendWholeWarps>::kRingBytes;
+    using Shared = AttendShared<D, kAttendWholeWarps>;
+    static_assert(Shared::kMergeBytes <= Shared::kRingBytes, "the merge takes the ring's room");
+    constexpr size_t smem = Shared::kRingBytes + kAttendWholeWarps * 16;
     auto *kernel = attention_kernel<T, D, NT, kAttendWholeWarps, true>;
     const cudaError_t err = allow_shared(kernel, smem, device, done_whole);
     if (err != cudaSuccess) return err;
@@ -171,7 +175,7 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
   p.piece_o = reinterpret_cast<float *>(w);
   p.piece_ml = reinterpret_cast<float *>(w + ml);
   p.piece_of = reinterpret_cast<int4 *>(w + of);
-  constexpr size_t smem = AttendShared<D, kAttendWarps>::kRingBytes;
+  constexpr size_t smem = AttendShared<D, kAttendWarps>::kRingBytes + AttendShared<D, kAttendWarps>::kMergeBytes;
   auto *kernel = attention_kernel<T, D, NT, kAttendWarps, false>;
   cudaError_t err = allow_shared(kernel, smem, device, done);
   if (err != cudaSuccess) return err;

@@ -70,7 +70,7 @@ __device__ __forceinline__ void table8(const void *table, int32_t type, int64_t 
 // table entries become one factor per element, z_lo = inv (x_lo c_lo + x_hi s_lo),
 // kept in registers over the token's heads.  kRotateBatch rounds of loads are in
 // flight before their first use.
-template <typename T, int D, bool Norm>
+template <typename T, int D, bool Norm, bool Full>
 __global__ void __launch_bounds__(kRotateThreads, kRotateCtas) rotate_store_kernel(const RotateArgs a, int rounds, int warps_per_token) {
   constexpr int kLanes = D / 16;
   constexpr int kHeads = 32 / kLanes;
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kRotateThreads, kRotateCtas) rotate_store_kern
   const int lane = threadIdx.x & 31;
   const int j = lane % kLanes, sub = lane / kLanes;
   const int half = a.rotary / 16;   // chunks in half the rotated part
-  const bool turns = j < half;
+  const bool turns = Full || j < half;   // Full: the whole head is rotated
   const int lo = (turns ? j : 2 * j) * 8, step = (turns ? half : 1) * 8;   // this lane's elements of a head: lo, lo + step
   const int q_rounds = (a.nq + kHeads - 1) / kHeads, k_rounds = (a.nkv + kHeads - 1) / kHeads;
   const int first = static_cast<int>(warp - t * warps_per_token) * rounds;
@@ -107,8 +107,13 @@ __global__ void __launch_bounds__(kRotateThreads, kRotateCtas) rotate_store_kern
   const int64_t pos = a.position[t];
   const int32_t slot = a.slot[t];
   const bool known = pos >= 0 && pos < a.rope_rows;
-  const bool stored = known && slot >= 0 && slot < a.num_blocks * a.block_size;
+  const bool stored = slot >= 0 && slot < a.num_blocks * a.block_size;
   T *q_dst = static_cast<T *>(a.q_out) + t * a.q_stride + lo;
+  if (!known) {   // uniform over the warp: zeros, nothing stored
+    for (int head = first * kHeads + sub; head < min(a.nq, last * kHeads); head += kHeads)
+      *reinterpret_cast<uint4 *>(q_dst + head * D) = *reinterpret_cast<uint4 *>(q_dst + head * D + step) = make_uint4(0, 0, 0, 0);
+    return;
+  }
   const int64_t cell =
       (stored ? (slot / a.block_size) * a.block_stride + static_cast<int64_t>(slot % a.block_size) * a.nkv * D : 0) + lo;
   // z_lo = x_lo c_lo + x_hi s_lo, z_hi = x_hi c_hi + x_lo s_hi (times the head's inverse norm)
@@ -119,7 +124,7 @@ __global__ void __launch_bounds__(kRotateThreads, kRotateCtas) rotate_store_kern
       c_lo[i] = c_hi[i] = make_float2(1.f, 1.f);
       s_lo[i] = s_hi[i] = make_float2(0.f, 0.f);
     }
-    if (known && turns) {
+    if (turns) {
       const int64_t at = pos * a.rotary + lo;
       table8(a.rope_cos, a.rope_dtype, at, c_lo);
       table8(a.rope_cos, a.rope_dtype, at + step, c_hi);
@@ -188,8 +193,8 @@ __global__ void __launch_bounds__(kRotateThreads, kRotateCtas) rotate_store_kern
       if (kind == 0) {
         if (head < a.nq) {
           T *dst = q_dst + head * D;
-          *reinterpret_cast<uint4 *>(dst) = known ? raw[b][0] : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4 *>(dst + step) = known ? raw[b][1] : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4 *>(dst) = raw[b][0];
+          *reinterpret_cast<uint4 *>(dst + step) = raw[b][1];
         }
       } else if (stored && head < a.nkv) {
         T *dst = static_cast<T *>(kind == 1 ? a.key_cache : a.value_cache) + cell + head * D;
