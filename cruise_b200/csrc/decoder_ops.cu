@@ -198,26 +198,79 @@ cudaError_t attention_of(const AttentionArgs &a, const AttentionShape &s, int de
 // ---- choose --------------------------------------------------------------------
 
 template <typename T>
+cudaLaunchConfig_t choose_launch(int rows, int ctas, size_t shared, cudaLaunchAttribute &attr) {
+  cudaLaunchConfig_t cfg{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.gridDim = dim3(ctas, rows);
+  cfg.blockDim = dim3(kChooseThreads);
+  cfg.dynamicSmemBytes = shared;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+// Clusters of 2^log CTAs that run at once: `alone` with an SM for each CTA, else
+// two to an SM.  Asked once per device (clusters lie within a group of SMs, and
+// the groups are not of one size: eight of 16 do not fit 148 SMs).
+template <typename T>
+int choose_fit(int log, bool alone, int device) {
+  static std::atomic<int> known[kMaxDevices][2][5];
+  const int ctas = 1 << log;
+  const bool cached = device >= 0 && device < kMaxDevices;
+  if (cached) {
+    const int n = known[device][alone ? 1 : 0][log].load(std::memory_order_relaxed);
+    if (n > 0) return n;
+  }
+  cudaLaunchAttribute attr{};
+  const cudaLaunchConfig_t cfg = choose_launch<T>(1, ctas, alone ? kChooseAlone : kChooseAlone / 2, attr);
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, choose_kernel<T>, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    return 1;
+  }
+  if (cached) known[device][alone ? 1 : 0][log].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+template <typename T>
 cudaError_t choose_typed(const ChooseArgs &a, int device, cudaStream_t stream) {
-  const int64_t entries = (a.history != nullptr ? a.history_width : 0) + static_cast<int64_t>(a.bias_token != nullptr ? a.bias_width : 0);
-  // as many CTAs per row as the SMs hold, one each: the call is as long as the
-  // chain of a CTA's steps, which a second one on the SM only stretches
-  const int sms = sm_count(device);
-  int ctas = 1;
-  while (ctas < kChooseMaxCluster &&
-         (choose_shared(choose_slice(a.vocab, ctas), entries) > 100 * 1024 ||
-          (static_cast<int64_t>(a.rows) * ctas * 2 <= sms && choose_slice(a.vocab, ctas) > 4096)))
-    ctas *= 2;
-  const int32_t slice = choose_slice(a.vocab, ctas);
   static std::atomic<uint64_t> done{0};
   cudaError_t err = allow_shared(choose_kernel<T>, kChooseShared, device, done, true);
   if (err != cudaSuccess) return err;
+  const int64_t entries = (a.history != nullptr ? a.history_width : 0) + static_cast<int64_t>(a.bias_token != nullptr ? a.bias_width : 0);
+  // CTAs per row: a CTA takes about 5 us for the chain of its steps and the
+  // marked tokens (as long as it streams 32768 fp32 logits), clusters 1 us more;
+  // two to an SM, the first takes 1.3 and the stream 1.6 times as long.  One row
+  // of 152064: 6.9 us with 16 CTAs, 12 with one; 17 rows: 8.2 with 4; 64 rows:
+  // 17 with 2, 26 with one.
+  int best = 0;
+  bool alone = false;
+  double least = 0;
+  for (int log = 0; log < 5; ++log) {
+    const int32_t slice = choose_slice(a.vocab, 1 << log);
+    const size_t shared = choose_shared(slice, entries);
+    if (shared > (log < 4 ? 100 * 1024 : kChooseShared)) continue;
+    const bool one = a.rows <= choose_fit<T>(log, true, device);
+    const int two = one ? a.rows : choose_fit<T>(log, false, device);
+    const double stream_cost = slice * (sizeof(T) / 4.0), chain = 32768 + (log > 0 ? 7000 : 0);
+    const double cost = (one ? chain + stream_cost : 1.3 * chain + 1.6 * stream_cost) * ((a.rows + two - 1) / two);
+    if (least == 0 || cost < least) {
+      least = cost;
+      best = log;
+      alone = one;
+    }
+  }
+  const int ctas = 1 << best;
+  const int32_t slice = choose_slice(a.vocab, ctas);
   // Where every CTA can have an SM of its own it takes more than half its shared
   // memory: a successor's CTAs, which come while this launch drains, would else
-  // settle two on the SMs it left idle (64 rows of 50257: 10.9 us, 9.4 so)
+  // settle two on the SMs it left idle (64 rows of 50257: 10.9 us, 8.8 so)
   const size_t shared = choose_shared(slice, entries);
-  return launch(choose_kernel<T>, dim3(ctas, a.rows), kChooseThreads,
-                static_cast<int64_t>(a.rows) * ctas <= sms ? std::max(shared, kChooseAlone) : shared, ctas, stream, a, slice);
+  return launch(choose_kernel<T>, dim3(ctas, a.rows), kChooseThreads, alone ? std::max(shared, kChooseAlone) : shared, ctas,
+                stream, a, slice);
 }
 
 // ---- errors --------------------------------------------------------------------
@@ -332,6 +385,7 @@ int32_t cruise_decoder_rotate_store(const void *qkv, int64_t qkv_stride, int32_t
       overlap(value_cache, cache_bytes, qkv, in_bytes) || overlap(q_out, out_bytes, key_cache, cache_bytes) ||
       overlap(q_out, out_bytes, value_cache, cache_bytes))
     return refuse("%s: q_out, the caches and qkv must not overlap", op);
+  if (key_cache == value_cache) return refuse("%s: the two caches must not be one", op);
   DeviceScope scope(device);
   if (scope.error != cudaSuccess) return report(scope.error, op);
   RotateArgs a{qkv, qkv_stride, tokens, num_heads, num_kv_heads, head_dim, dtype, position, slot, q_norm, k_norm, eps,
@@ -431,7 +485,7 @@ int32_t cruise_decoder_choose(const void *logits, int64_t logits_stride, int32_t
   if (rows < 0 || rows > 65535 || vocab < 1 || vocab > kChooseMaxVocab)
     return refuse("%s: %d rows of %d logits (at most 65535 rows of 1 to %d)", op, rows, vocab, kChooseMaxVocab);
   const int64_t entries = (history != nullptr ? history_width : 0) + static_cast<int64_t>(bias_token != nullptr ? bias_width : 0);
-  if (choose_shared(choose_slice(vocab, kChooseMaxCluster), entries) > kChooseShared)
+  if (entries > kMaxIndex || choose_shared(choose_slice(vocab, kChooseMaxCluster), entries) > kChooseShared)
     return refuse("%s: a history and bias list of %lld entries with %d logits (at most 20000 beyond 390000 logits)", op,
                   static_cast<long long>(entries), vocab);
   if (dtype < kBf16 || dtype > kFp32) return refuse("%s: dtype %d (0 bf16, 1 fp16 or 2 fp32)", op, dtype);
@@ -458,6 +512,16 @@ int32_t cruise_decoder_choose(const void *logits, int64_t logits_stride, int32_t
     if (!in_place && overlap(processed, extent(rows, processed_stride, vocab, 4), logits, logits_bytes))
       return refuse("%s: processed must be the fp32 logits themselves or not overlap them", op);
   }
+  const int64_t processed_bytes = processed != nullptr ? extent(rows, processed_stride, vocab, 4) : 0;
+  const int64_t history_bytes = history != nullptr ? extent(rows, history_stride, history_width, 4) : 0;
+  const int64_t allowed_bytes = allowed != nullptr ? extent(rows, allowed_stride, (vocab + 31) / 32, 4) : 0;
+  const int64_t bias_bytes = bias_token != nullptr ? extent(rows, bias_stride, bias_width, 4) : 0;
+  if (overlap(processed, processed_bytes, history, history_bytes) || overlap(processed, processed_bytes, allowed, allowed_bytes) ||
+      overlap(processed, processed_bytes, bias_token, bias_bytes) || overlap(processed, processed_bytes, bias_value, bias_bytes) ||
+      overlap(token, 8ll * rows, logits, logits_bytes) || overlap(token, 8ll * rows, history, history_bytes) ||
+      overlap(token, 8ll * rows, processed, processed_bytes) || overlap(token, 8ll * rows, allowed, allowed_bytes) ||
+      (append != 0 && (overlap(history, history_bytes, logits, logits_bytes) || overlap(history, history_bytes, allowed, allowed_bytes))))
+    return refuse("%s: token, processed and the history must not overlap the inputs", op);
   DeviceScope scope(device);
   if (scope.error != cudaSuccess) return report(scope.error, op);
   ChooseArgs a{logits, logits_stride, rows, vocab, dtype, active, history, history_stride, history_width, prompt_len,

@@ -1259,6 +1259,11 @@ int32_t run_decoder_step_paged(Engine *e, const PagedStep &s) {
       return reject("every tensor must be device memory on the engine's device");
     }
   }
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(s.stream, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone) {
+    cudaGetLastError();
+    return reject("a step waits for its result and cannot be captured");
+  }
   int32_t rc = prefill_prepare(e);
   if (rc != 0) {
     prefill_release(e);

@@ -299,7 +299,8 @@ int32_t cruise_decoder_step(void *engine, const int64_t *token,
  * rounding: cruise_decoder_step gives the same values as f32).  Rounds where the
  * decoder does, but for the attention's scores and probabilities and the
  * rotation, which stay in fp32.
- * Waits for what `stream` holds, and returns when the step has completed.
+ * Waits for what `stream` holds, and returns when the step has completed (so
+ * a capturing stream is refused).
  * Returns 0, -1 for invalid arguments, -2 when a projection could not be
  * launched, -3 when a device-side wait gave up, -4 for a tensor-parallel
  * engine, or a CUDA error code; cruise_epoch_last_error explains them. */

@@ -44,7 +44,7 @@ def call(name: str, arguments: dict) -> tuple[int, str]:
     (dict(num_blocks=0), "blocks"), (dict(num_blocks=1 << 30), "below 2^31"), (dict(qkv_stride=504), "stride"),
     (dict(q_stride=257), "multiples of 8"), (dict(block_stride=1024), "stride"), (dict(qkv=None), "NULL"),
     (dict(slot=None), "NULL"), (dict(qkv=at(0) + 8), "aligned"), (dict(q_out=at(0) + 64), "overlap"),
-    (dict(key_cache=at(0)), "overlap"), (dict(q_out=at(6) + 2048), "overlap"),
+    (dict(key_cache=at(0)), "overlap"), (dict(key_cache=at(7)), "must not be one"), (dict(q_out=at(6) + 2048), "overlap"),
 ])
 def test_rotate_store_refuses(change, reason):
     rc, why = call("cruise_decoder_rotate_store", {**ROTATE, **change})
@@ -82,7 +82,8 @@ def test_attention_refuses(change, reason):
     (dict(bias_token=at(6), bias_value=at(7), bias_len=at(8), bias_width=4, bias_stride=3), "bias list"),
     (dict(allowed=at(6), allowed_stride=3), "stride"), (dict(processed=at(6), processed_stride=99), "stride"),
     (dict(processed=at(0) + 64, processed_stride=100), "overlap"),
-    (dict(processed=at(0), processed_stride=104), "overlap"), (dict(token=None), "NULL"), (dict(logits=None), "NULL"),
+    (dict(processed=at(0), processed_stride=104), "overlap"), (dict(processed=at(1) - 64, processed_stride=100), "overlap"),
+    (dict(token=at(1)), "overlap"), (dict(allowed=at(4) - 32, allowed_stride=4), "overlap"), (dict(token=None), "NULL"), (dict(logits=None), "NULL"),
     (dict(logits=at(0) + 2), "aligned"), (dict(token=at(4) + 4), "aligned"),
 ])
 def test_choose_refuses(change, reason):

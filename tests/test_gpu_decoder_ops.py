@@ -627,6 +627,62 @@ def test_captured_attention_follows_its_inputs():
             assert torch.equal(out, want)
 
 
+def test_captured_calls_behind_copies_memsets_and_joins():
+    """Captured behind a memset, a copy and a join of two streams, each call
+    still waits for what it reads."""
+    from cruise_b200.decoder_ops import choose, paged_attention, rotate_store
+
+    case = attend_case([700, 90], 8, 2, 64, BF16, seed=33)
+    rot, keep = rotate_case(40, 4, 2, 64, BF16, seed=34)
+    pick = dict(logits=randn(gen(35), 3, 5000))
+    source = {name: t.clone() for name, t in (("q", case["q"]), ("qkv", rot["qkv"]), ("logits", pick["logits"]))}
+    out = [torch.empty_like(case["q"]), torch.empty(40, 4, 64, dtype=BF16, device="cuda"), torch.empty(3, dtype=torch.int64, device="cuda")]
+
+    def body(side):
+        case["q"].zero_()
+        paged_attention(*case.values(), out=out[0])            # behind a memset: uniform weights
+        case["q"].copy_(source["q"])
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            rot["qkv"].copy_(source["qkv"])
+            rotate_store(*rot.values(), **keep, out=out[1])    # behind a copy, on another stream
+            pick["logits"].copy_(source["logits"])
+        torch.cuda.current_stream().wait_stream(side)
+        choose(**pick, out=out[2])                             # behind a join
+        paged_attention(*case.values(), out=out[0])
+
+    side = torch.cuda.Stream()
+    body(side)
+    torch.cuda.synchronize()
+    want = [t.clone() for t in out]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        body(side)
+    for _ in range(5):
+        for t in (*out, case["q"], rot["qkv"]):
+            t.fill_(1)
+        pick["logits"].fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, wanted in zip(out, want):
+            assert torch.equal(got, wanted)
+
+
+def test_calls_one_after_another_wait_for_each_other():
+    """A chain of calls that each read what the one before wrote, without a pause."""
+    from cruise_b200.decoder_ops import paged_attention
+
+    case = attend_case([900, 33, 128], 4, 2, 64, FP16, width=80, seed=36)
+    slow = case["q"].clone()
+    for _ in range(30):
+        slow = paged_attention(slow, *list(case.values())[1:])
+        torch.cuda.synchronize()
+    fast = case["q"].clone()
+    for _ in range(30):
+        fast = paged_attention(fast, *list(case.values())[1:])
+    assert torch.equal(fast, slow)
+
+
 # ---- a run of the three, as a decode loop uses them ----------------------------------------
 
 class DecodeLoop:

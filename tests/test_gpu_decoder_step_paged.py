@@ -90,17 +90,19 @@ def test_paged_step_matches_the_oracle_step(cuda_ok, geometry, block_size, block
     engine.close()
 
 
-def test_paged_step_agrees_with_the_resident_step(cuda_ok):
+@pytest.mark.parametrize("geometry", ["tiny", "7b-2l"])
+def test_paged_step_agrees_with_the_resident_step(cuda_ok, geometry):
     """The same caches, tables and inputs through both steps."""
     from cruise_b200.engine import EpochEngine
-    from cruise_b200.model_config import TINY
+    from cruise_b200.model_config import QWEN25_7B, TINY
 
-    engine = EpochEngine(TINY)
+    cfg = TINY if geometry == "tiny" else replace(QWEN25_7B, name="qwen2.5-7b-2l", num_layers=2)
+    engine = EpochEngine(cfg)
     engine.init_synthetic(0)
-    sc = make_scenario(vocab=TINY.vocab, seed=9)
-    for inputs in prefill_epochs(sc, TINY.block_size, TINY.vocab):
+    sc = make_scenario(vocab=cfg.vocab, seed=9, token_high=min(cfg.vocab, 151643))
+    for inputs in prefill_epochs(sc, cfg.block_size, cfg.vocab):
         assert engine.run(**inputs).status == 0
-    inputs = decode_inputs(sc, TINY.block_size)
+    inputs = decode_inputs(sc, cfg.block_size)
     rows = [r for r in range(4) if inputs["active"][r]]
     caches = [c.cuda() for c in engine.read_kv()]
     want, _ = engine.decoder_step(inputs["token"], inputs["position"], inputs["seq_len"], inputs["slot"], inputs["active"],
@@ -177,6 +179,10 @@ def test_paged_step_refuses(cuda_ok):
     with pytest.raises(EngineError, match="rows outside"):
         engine.decoder_step_paged(torch.zeros(many, dtype=torch.int64, device="cuda"), torch.zeros(many, dtype=torch.int64, device="cuda"),
                                   torch.zeros(many, 1, dtype=torch.int32, device="cuda"), args["key"], args["value"])
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(EngineError, match="captured"):
+        with torch.cuda.graph(graph):
+            engine.decoder_step_paged(**args)
     # rows that do not exist are inactive: nothing is stored
     before = args["key"].clone()
     args.update(token=torch.tensor([-1, 4096, 5, 6], device="cuda"), position=torch.tensor([0, 0, -3, 64], device="cuda"))
