@@ -21,9 +21,9 @@ namespace cruise {
 namespace ops {
 
 constexpr int kAttendKeys = 16;      // keys of a warp's step
-constexpr int kAttendStages = 3;
 constexpr int kAttendWarps = 4;      // warps of a CTA that shares the work with the others
-constexpr int kAttendWholeWarps = 8; // warps of a CTA that takes one whole unit
+constexpr int kAttendWholeWarps = 8; // warps of a CTA of a cluster that takes one unit
+constexpr int kAttendRanks = 16;     // CTAs of such a cluster, at most
 constexpr int kJoinThreads = 512;
 constexpr int kJoinBatch = 6;        // pieces a thread has in flight
 
@@ -54,15 +54,19 @@ struct AttentionPlan {
   // where units outnumber the CTAs by CTA [grid], for the unit in its slot 1.
   int4 *piece_of;
   int32_t by_unit;
+  int32_t ranks;       // CTAs of a cluster that takes one unit
 };
 
 template <int D, int Warps>
 struct AttendShared {
+  static constexpr int kStages = Warps == kAttendWholeWarps && D == 64 ? 6 : 3;   // steps of a warp's ring
   static constexpr int kRowBytes = D * 2;
   static constexpr int kStageBytes = 2 * kAttendKeys * kRowBytes;   // K then V
-  static constexpr int kRingBytes = Warps * kAttendStages * kStageBytes;
+  static constexpr int kRingBytes = Warps * kStages * kStageBytes;
   static constexpr int kMergeStride = D + 4;                        // fp32; no bank conflicts for the fragment stores
   static constexpr int kMergeBytes = Warps * 8 * kMergeStride * 4;  // 8 heads of every warp
+  // what a cluster's CTAs send one another: m and l of every rank and head, and of O the slice this CTA joins
+  static constexpr int kInboxBytes(int heads) { return kAttendRanks * heads * 8 + (heads * (D / 4) + kAttendRanks) * 16; }
 };
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -106,6 +110,7 @@ __host__ __device__ __forceinline__ int row_tiles(int length) {
 template <typename T, int D, int NT, int Warps, bool Whole>
 __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attention_kernel(const AttentionPlan p) {
   using S = AttendShared<D, Warps>;
+  constexpr int kAttendStages = S::kStages;
   constexpr int kAttendThreads = Warps * 32, kAttendTile = Warps * kAttendKeys;
   // The ring, then the merge's room (a whole unit's CTA merges in the ring).  Two
   // CTAs of head size 128 take the SM's shared memory to the last byte, so the
@@ -116,9 +121,9 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
   auto factor = [&](int w, int h) -> float & { return NT == 1 ? merge_f_room[w * 8 + h] : merge_ml[w][h][0]; };
   uint32_t *const words = reinterpret_cast<uint32_t *>(ring + S::kRingBytes);
   auto word = [&](int line, int i) -> uint32_t & {   // word i < 4 of 8 * Warps lines
-    return Whole ? words[line * 4 + i] : words[line * S::kMergeStride + D + i];
+    return Whole ? words[line * 8 + i] : words[line * S::kMergeStride + D + i];
   };
-  static_assert(kAttendStages <= 4, "a line holds a warp's masks");
+  static_assert(kAttendStages <= (Whole ? 8 : 4), "a line holds a warp's masks");
   constexpr int kChunks = D / 8;   // 16-byte chunks of a row
   const AttentionArgs &a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -129,9 +134,11 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
   // set-up, then its tiles) --
   constexpr int kSetup = attend_setup(D);
   int row, off = 0, left = 1, length0;
+  const int ranks = Whole ? p.ranks : 1, rank = Whole ? static_cast<int>(blockIdx.x) : 0;
   if constexpr (Whole) {
-    row = blockIdx.x / p.units;
+    row = blockIdx.z;
     length0 = row_length(p, row);
+    if (ranks > 1) cluster_arrive();   // every CTA of the cluster runs before its shared memory is written
   } else {
     const int per = (a.rows + kAttendThreads - 1) / kAttendThreads;
     const int r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
@@ -202,9 +209,9 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
       s.length = c.length;
       s.n = row_tiles<Warps>(s.length);
       if constexpr (Whole) {
-        s.unit = blockIdx.x - c.row * p.units;   // (known before the length)
-        s.t0 = 0;
-        s.count = s.n;
+        s.unit = blockIdx.y;
+        s.t0 = rank;   // and every `ranks`-th tile from there, so that the first is known before the length
+        s.count = s.n > rank ? (s.n - rank + ranks - 1) / ranks : 0;
         c.left = 0;
         return true;
       } else {
@@ -239,7 +246,7 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
   // copies of a step do not wait for the table) and without the row's length
   // (the first step waits for one load, not two)
   auto block_of = [&](int i) {
-    const int t = (from.t0 + i) * kAttendTile + warp * kAttendKeys + lane;
+    const int t = (from.t0 + i * ranks) * kAttendTile + warp * kAttendKeys + lane;
     if (lane >= kAttendKeys || t >= p.capacity) return -1;
     return table[p.block_shift >= 0 ? t >> p.block_shift : t / a.block_size];
   };
@@ -253,13 +260,14 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
         vsrc = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.value_cache) + kvh * D) + lane % kChunks;
         load_tile = 0;
         next_block = block_of(0);
+        if constexpr (Whole) loading = from.count > 0;
       }
     }
     uint32_t mask = 0;
     if (loading) {
       const int id = next_block;
       next_block = block_of(load_tile + 1);
-      const int t = (from.t0 + load_tile) * kAttendTile + warp * kAttendKeys + lane;
+      const int t = (from.t0 + load_tile * ranks) * kAttendTile + warp * kAttendKeys + lane;
       const bool live = t < from.length && id >= 0 && id < a.num_blocks;
       uint32_t at = 0;   // the key's row, in 16-byte chunks of the cache
       if (live) {
@@ -403,7 +411,12 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
       }
     }
     __syncthreads();   // every warp is done with its products, and with the merge before this one
-    const bool whole = t0 == 0 && count == n;
+    const bool whole = Whole ? ranks == 1 : t0 == 0 && count == n;
+    // the cluster's inbox: [rank][head] (m, l), then [rank][join_each] four dimensions of O
+    float2 *const inbox_ml = reinterpret_cast<float2 *>(words + Warps * 8);
+    float4 *const inbox_o = reinterpret_cast<float4 *>(inbox_ml + kAttendRanks * NT * 8);
+    const int join_each = Whole ? (heads * (D / 4) + ranks - 1) / ranks : 0;
+    if (Whole && !whole) cluster_wait();
     const int64_t piece = 2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0);
     if (tid < (heads * Warps + 31) / 32 * 32) {   // whole warps: a lane per (head, warp)
       // the head's maximum and sum over the warps, each warp's factor, lse
@@ -420,7 +433,9 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
       if (live) {
         // a whole unit is divided here; no key with a weight gives zeros and log 0
         factor(w, h) = !whole ? f : sum == 0.f ? 0.f : f / sum;
-        if (w == 0) {
+        if (Whole && !whole) {
+          for (int r = w; r < ranks; r += Warps) store_cluster(inbox_ml + rank * (NT * 8) + h, r, make_float2(top, sum));
+        } else if (w == 0) {
           if (!whole) {
             *reinterpret_cast<float2 *>(p.piece_ml + (piece * (NT * 8) + h) * 2) = make_float2(top, sum);
           } else if (a.lse != nullptr) {
@@ -456,12 +471,42 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
         if (whole) {
           *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + row_now * a.out_stride + static_cast<int64_t>(head0 + nt * 8 + h) * D + c) =
               make_uint2(Element<T>::pack(o.x, o.y), Element<T>::pack(o.z, o.w));
+        } else if constexpr (Whole) {
+          const int to = (nt * (8 * D / 4) + i) / join_each;
+          store_cluster(inbox_o + rank * join_each + (nt * (8 * D / 4) + i - to * join_each), to, o);
         } else {
           *reinterpret_cast<float4 *>(p.piece_o + piece * (NT * 8 * D) + (nt * 8 + h) * D + c) = o;
         }
       }
     }
-    if (NT > 1) __syncthreads();   // the factors have been read
+    if (Whole && !whole) {   // every CTA joins its slice of the heads' dimensions
+      cluster_arrive();
+      cluster_wait();
+      const int i = rank * join_each + tid, h = i / (D / 4), c = i % (D / 4) * 4;
+      if (tid < join_each && h < heads) {
+        float top = -INFINITY;
+        for (int r = 0; r < ranks; ++r) top = fmaxf(top, inbox_ml[r * (NT * 8) + h].x);
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r = 0; r < ranks; ++r) {
+          const float2 ml = inbox_ml[r * (NT * 8) + h];
+          const float4 v = inbox_o[r * join_each + tid];
+          const float f = exp2f(ml.x - base);
+          sum = fmaf(ml.y, f, sum);
+          o.x = fmaf(v.x, f, o.x);
+          o.y = fmaf(v.y, f, o.y);
+          o.z = fmaf(v.z, f, o.z);
+          o.w = fmaf(v.w, f, o.w);
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + row_now * a.out_stride + static_cast<int64_t>(head0 + h) * D + c) =
+            make_uint2(Element<T>::pack(o.x * inv, o.y * inv), Element<T>::pack(o.z * inv, o.w * inv));
+        if (c == 0 && a.lse != nullptr)
+          a.lse[static_cast<int64_t>(row_now) * a.nq + head0 + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+      }
+    }
+    if (NT > 1 && !Whole) __syncthreads();   // the factors have been read
     if (!Whole && t0 == 0) {
       const int4 of = make_int4(row_now, unit, whole ? 0 : 1 + (n - count + share_work - 1) / share_work, blockIdx.x);
       if (p.by_unit) {

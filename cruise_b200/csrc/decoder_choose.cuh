@@ -73,16 +73,6 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   return r;
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-
-// Stores a word into the shared memory of CTA `rank` of the cluster.
-__device__ __forceinline__ void store_cluster(void *local, uint32_t rank, uint32_t v) {
-  uint32_t addr;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(local)), "r"(rank));
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-
 // Tokens of a CTA's slice: a multiple of 32, so that slices share no mask word.
 inline int32_t choose_slice(int32_t vocab, int32_t ctas) { return ((vocab + ctas - 1) / ctas + 31) / 32 * 32; }
 

@@ -20,6 +20,28 @@ __device__ __forceinline__ void follow_predecessor() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// The CTAs of a cluster: a barrier in two halves, and their shared memory.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// The address in CTA `rank`'s shared memory of what `local` is in this one's.
+__device__ __forceinline__ uint32_t cluster_address(const void *local, uint32_t rank) {
+  uint32_t addr;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(local)), "r"(rank));
+  return addr;
+}
+__device__ __forceinline__ void store_cluster(void *local, uint32_t rank, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_address(local, rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ void store_cluster(void *local, uint32_t rank, float2 v) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_address(local, rank)), "f"(v.x), "f"(v.y) : "memory");
+}
+__device__ __forceinline__ void store_cluster(void *local, uint32_t rank, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_address(local, rank)), "f"(v.x), "f"(v.y),
+               "f"(v.z), "f"(v.w)
+               : "memory");
+}
+
 template <typename T>
 struct Element;
 

@@ -91,6 +91,21 @@ cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, size_t sha
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// What an occupancy query takes of such a launch.
+cudaLaunchConfig_t cluster_launch(dim3 grid, int threads, size_t shared, int cluster, cudaLaunchAttribute &attr) {
+  cudaLaunchConfig_t cfg{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = shared;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
 // ---- rotate_store --------------------------------------------------------------
 
 template <typename T, int D>
@@ -112,13 +127,49 @@ cudaError_t rotate_typed(const RotateArgs &a, int device, cudaStream_t stream) {
 
 // ---- paged_attention -----------------------------------------------------------
 
-// How the heads of a KV head form units of at most 16, and whether a unit is
-// worth splitting over the length.
+// How the heads of a KV head form units of at most 16, and how many CTAs take a
+// unit as a cluster (0: the units are split over all CTAs).
 struct AttentionShape {
   int32_t groups, chunks, chunk, units;
-  bool whole;
+  int32_t ranks;
   int grid;   // CTAs of the split form
 };
+
+template <typename T, int D, int NT>
+cudaError_t allow_whole(int device, size_t *bytes) {
+  using Shared = AttendShared<D, kAttendWholeWarps>;
+  static_assert(Shared::kMergeBytes <= Shared::kRingBytes, "the merge takes the ring's room");
+  static std::atomic<uint64_t> done{0};
+  *bytes = Shared::kRingBytes + kAttendWholeWarps * 32 + Shared::kInboxBytes(NT * 8);
+  return allow_shared(attention_kernel<T, D, NT, kAttendWholeWarps, true>, *bytes, device, done, true);
+}
+
+// Clusters of `ranks` CTAs, an SM each, that run at once (the types' kernels do
+// not differ in this).
+template <int D, int NT>
+int attention_fit(int ranks, int device) {
+  static std::atomic<int> known[kMaxDevices][kAttendRanks + 1];
+  const bool cached = device >= 0 && device < kMaxDevices;
+  if (ranks == 1) return sm_count(device);
+  if (cached) {
+    const int n = known[device][ranks].load(std::memory_order_relaxed);
+    if (n > 0) return n;
+  }
+  DeviceScope scope(device);
+  size_t shared = 0;
+  int n = 0;
+  if (scope.error == cudaSuccess && allow_whole<__nv_bfloat16, D, NT>(device, &shared) == cudaSuccess) {
+    cudaLaunchAttribute attr{};
+    const cudaLaunchConfig_t cfg = cluster_launch(dim3(ranks), kAttendWholeWarps * 32, shared, ranks, attr);
+    if (cudaOccupancyMaxActiveClusters(&n, attention_kernel<__nv_bfloat16, D, NT, kAttendWholeWarps, true>, &cfg) != cudaSuccess) n = 0;
+  }
+  if (n <= 0) {
+    cudaGetLastError();
+    return sm_count(device) / 16 * (16 / ranks);
+  }
+  if (cached) known[device][ranks].store(n, std::memory_order_relaxed);
+  return n;
+}
 
 AttentionShape attention_shape(int32_t rows, int32_t nq, int32_t nkv, int32_t d, int64_t capacity, int device) {
   AttentionShape s;
@@ -126,9 +177,17 @@ AttentionShape attention_shape(int32_t rows, int32_t nq, int32_t nkv, int32_t d,
   s.chunks = (s.groups + 15) / 16;
   s.chunk = (s.groups + s.chunks - 1) / s.chunks;
   s.units = nkv * s.chunks;
-  // few short rows: one CTA per unit and no second kernel
   const int sms = sm_count(device);
-  s.whole = capacity <= 8 * kAttendWholeWarps * kAttendKeys && static_cast<int64_t>(rows) * s.units <= sms;
+  const int64_t units = std::max<int64_t>(1, static_cast<int64_t>(rows) * s.units);
+  s.ranks = 0;
+  if (units <= sms) {
+    const auto fit = d == 128 ? (s.chunk <= 8 ? attention_fit<128, 1> : attention_fit<128, 2>)
+                              : (s.chunk <= 8 ? attention_fit<64, 1> : attention_fit<64, 2>);
+    const int64_t tiles = std::max<int64_t>(1, (capacity + kAttendWholeWarps * kAttendKeys - 1) / (kAttendWholeWarps * kAttendKeys));
+    int ranks = tiles <= 2 ? 1 : static_cast<int>(std::min<int64_t>({sms / units, tiles, kAttendRanks}));
+    while (ranks > 1 && fit(ranks, device) < units) --ranks;
+    if (tiles <= 8 * ranks) s.ranks = ranks;
+  }
   s.grid = sms * attend_ctas(d);
   return s;
 }
@@ -158,15 +217,14 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
   p.block_chunks = static_cast<uint32_t>(a.block_stride / 8);
   p.slot_chunks = static_cast<uint32_t>(a.nkv * D / 8);
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  static std::atomic<uint64_t> done{0}, done_whole{0};
-  if (s.whole) {
-    using Shared = AttendShared<D, kAttendWholeWarps>;
-    static_assert(Shared::kMergeBytes <= Shared::kRingBytes, "the merge takes the ring's room");
-    constexpr size_t smem = Shared::kRingBytes + kAttendWholeWarps * 16;
-    auto *kernel = attention_kernel<T, D, NT, kAttendWholeWarps, true>;
-    const cudaError_t err = allow_shared(kernel, smem, device, done_whole);
+  static std::atomic<uint64_t> done{0};
+  if (s.ranks > 0) {
+    p.ranks = s.ranks;
+    size_t smem = 0;
+    const cudaError_t err = allow_whole<T, D, NT>(device, &smem);
     if (err != cudaSuccess) return err;
-    return launch(kernel, dim3(static_cast<unsigned>(a.rows) * s.units), kAttendWholeWarps * 32, smem, 1, stream, p);
+    return launch(attention_kernel<T, D, NT, kAttendWholeWarps, true>, dim3(s.ranks, s.units, a.rows), kAttendWholeWarps * 32, smem,
+                  s.ranks, stream, p);
   }
   p.by_unit = static_cast<int64_t>(a.rows) * s.units <= s.grid ? 1 : 0;
   size_t ml = 0, of = 0;
@@ -197,21 +255,6 @@ cudaError_t attention_of(const AttentionArgs &a, const AttentionShape &s, int de
 
 // ---- choose --------------------------------------------------------------------
 
-template <typename T>
-cudaLaunchConfig_t choose_launch(int rows, int ctas, size_t shared, cudaLaunchAttribute &attr) {
-  cudaLaunchConfig_t cfg{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(ctas);
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.gridDim = dim3(ctas, rows);
-  cfg.blockDim = dim3(kChooseThreads);
-  cfg.dynamicSmemBytes = shared;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cfg;
-}
-
 // Clusters of 2^log CTAs that run at once: `alone` with an SM for each CTA, else
 // two to an SM.  Asked once per device (clusters lie within a group of SMs, and
 // the groups are not of one size: eight of 16 do not fit 148 SMs).
@@ -225,7 +268,7 @@ int choose_fit(int log, bool alone, int device) {
     if (n > 0) return n;
   }
   cudaLaunchAttribute attr{};
-  const cudaLaunchConfig_t cfg = choose_launch<T>(1, ctas, alone ? kChooseAlone : kChooseAlone / 2, attr);
+  const cudaLaunchConfig_t cfg = cluster_launch(dim3(ctas), kChooseThreads, alone ? kChooseAlone : kChooseAlone / 2, ctas, attr);
   int n = 0;
   if (cudaOccupancyMaxActiveClusters(&n, choose_kernel<T>, &cfg) != cudaSuccess || n <= 0) {
     cudaGetLastError();
@@ -317,7 +360,7 @@ cudaError_t launch_rotate_store(const RotateArgs &a, int device, cudaStream_t st
 
 int64_t attention_workspace(int32_t rows, int32_t nq, int32_t nkv, int32_t d, int64_t capacity, int device) {
   const AttentionShape s = attention_shape(rows, nq, nkv, d, capacity, device);
-  if (s.whole) return 0;
+  if (s.ranks > 0) return 0;
   return static_cast<int64_t>(pieces_bytes(s.grid, s.chunk <= 8 ? 8 : 16, d, nullptr, nullptr));
 }
 

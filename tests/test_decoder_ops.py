@@ -60,11 +60,15 @@ def test_rotate_store_refuses(change, reason):
     (dict(num_blocks=1 << 20, block_stride=1 << 16), "2^35"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(out=None), "NULL"),
     (dict(block_table=None), "NULL"), (dict(q=at(0) + 2), "aligned"), (dict(out=at(0)), "overlap"),
     (dict(out=at(2) + 4096), "overlap"), (dict(lse=at(5) + 16), "overlap"), (dict(lse=at(4)), "overlap"),
-    (dict(table_width=64, table_stride=64), "workspace"),
-    (dict(table_width=64, table_stride=64, workspace=at(9), workspace_bytes=64), "workspace"),
-    (dict(table_width=64, table_stride=64, workspace=at(1) - 4096, workspace_bytes=1 << 40), "workspace must not"),
+    (dict(table_width=1 << 16, table_stride=1 << 16), "workspace"),
+    (dict(table_width=1 << 16, table_stride=1 << 16, workspace=at(9), workspace_bytes=64), "workspace"),
+    (dict(table_width=1 << 16, table_stride=1 << 16, workspace=at(1) - 4096, workspace_bytes=1 << 40), "workspace must not"),
 ])
 def test_attention_refuses(change, reason):
+    if "workspace" in reason:   # long rows are split whatever the device, and the pieces need room
+        lib, a = _lib.load(), {**ATTEND, **change}
+        assert lib.cruise_decoder_attention_workspace(a["rows"], a["num_heads"], a["num_kv_heads"], a["head_dim"],
+                                                      a["table_width"] * a["block_size"], a["device"]) > 64
     rc, why = call("cruise_decoder_attention", {**ATTEND, **change})
     if torch.cuda.is_available() or "workspace" not in reason:
         assert rc == -1 and reason in why, (rc, why)

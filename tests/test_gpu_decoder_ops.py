@@ -191,6 +191,16 @@ def check_attend(case, **keep):
     ([1] * 150 + [2500], 4, 2, 64, 16, None),       # more rows than threads of a CTA
     ([0, 0, 0], 4, 2, 128, 128, 8),
     ([10000], 12, 4, 128, 128, 1024),               # a table far wider than the row
+    ([1, 0, 127, 128, 129, 1000, 2048], 6, 2, 128, 64, None),   # ten CTAs a unit, more than some rows have tiles
+    ([383, 384, 385, 0], 14, 2, 64, 32, None),
+    ([256, 257, 300], 16, 1, 128, 16, None),
+    ([16384, 5], 8, 1, 128, 128, None),
+    ([1024] * 36 + [0], 28, 4, 128, 128, None),     # one CTA for each unit, and for each SM
+    ([513, 0, 1, 2000, 64, 5000], 7, 1, 128, 16, 2000),         # wide tables: units split over all CTAs
+    ([3000, 1, 0, 777], 32, 8, 64, 24, 1000),
+    ([1025] * 5, 16, 1, 64, 32, 600),
+    ([700, 20, 1300], 40, 2, 128, 128, 150),
+    ([900, 0, 4097], 33, 1, 64, 48, 400),
 ])
 def test_paged_attention(lens, nq, nkv, d, block, width, dtype):
     check_attend(attend_case(lens, nq, nkv, d, dtype, block=block, width=width, seed=len(lens)))
@@ -206,7 +216,7 @@ def test_paged_attention_sharp_and_scaled():
     check_attend(attend_case([600, 37], 8, 2, 64, BF16, seed=2), scale=0.0)
 
 
-@pytest.mark.parametrize("width", [4, 64])
+@pytest.mark.parametrize("width", [4, 64, 2000])
 def test_paged_attention_ignores_what_is_masked(width):
     """NaN and infinities behind a row's length, in blocks of nobody and behind
     invalid table entries do not reach the outputs."""
@@ -228,7 +238,7 @@ def test_paged_attention_ignores_what_is_masked(width):
         assert torch.equal(paged_attention(*case.values()), clean)
 
 
-@pytest.mark.parametrize("width", [2, 80])
+@pytest.mark.parametrize("width", [2, 80, 2000])
 def test_paged_attention_no_valid_block(width):
     case = attend_case([20, 30], 4, 2, 128, BF16, block=16, width=width, seed=4)
     case["block_table"][1] = -1
@@ -236,7 +246,7 @@ def test_paged_attention_no_valid_block(width):
     assert not out[1].any()
 
 
-@pytest.mark.parametrize("width", [4, 64])
+@pytest.mark.parametrize("width", [4, 64, 2000])
 def test_paged_attention_propagates_what_is_attended(width):
     from cruise_b200.decoder_ops import paged_attention
 
@@ -571,7 +581,7 @@ def test_overlapping_calls_do_not_meet():
 
     from cruise_b200.decoder_ops import paged_attention
 
-    cases = [attend_case([9000 - 37 * i], 8, 2, 64, BF16, seed=22 + i) for i in range(4)]
+    cases = [attend_case([9000 - 37 * i], 8, 2, 64, BF16, width=2000, seed=22 + i) for i in range(4)]
     wants = [paged_attention(*c.values()) for c in cases]
     torch.cuda.synchronize()
     bad = []
@@ -599,7 +609,7 @@ def test_captured_attention_follows_its_inputs():
     that replay at once on two streams do not share a workspace."""
     from cruise_b200.decoder_ops import paged_attention
 
-    cases = [attend_case([2000, 17, 900], 8, 2, 64, BF16, seed=30 + i) for i in range(2)]
+    cases = [attend_case([2000, 17, 900], 8, 2, 64, BF16, width=2000, seed=30 + i) for i in range(2)]
     outs = [torch.empty_like(c["q"]) for c in cases]
     graphs = []
     for case, out in zip(cases, outs):
@@ -668,11 +678,12 @@ def test_captured_calls_behind_copies_memsets_and_joins():
             assert torch.equal(got, wanted)
 
 
-def test_calls_one_after_another_wait_for_each_other():
+@pytest.mark.parametrize("width", [80, 2000])
+def test_calls_one_after_another_wait_for_each_other(width):
     """A chain of calls that each read what the one before wrote, without a pause."""
     from cruise_b200.decoder_ops import paged_attention
 
-    case = attend_case([900, 33, 128], 4, 2, 64, FP16, width=80, seed=36)
+    case = attend_case([900, 33, 128], 4, 2, 64, FP16, width=width, seed=36)
     slow = case["q"].clone()
     for _ in range(30):
         slow = paged_attention(slow, *list(case.values())[1:])
