@@ -57,6 +57,10 @@ struct AttentionPlan {
   int32_t ranks;       // CTAs of a cluster that takes one unit
 };
 
+// How the work meets the CTAs: units split over all of them, a unit for each, or
+// a unit for a cluster of them.
+enum class AttendForm { kSplit, kWhole, kCluster };
+
 template <int D, int Warps>
 struct AttendShared {
   static constexpr int kStages = Warps == kAttendWholeWarps && D == 64 ? 6 : 3;   // steps of a warp's ring
@@ -107,9 +111,10 @@ __host__ __device__ __forceinline__ int row_tiles(int length) {
   return length <= kTile ? 1 : (length + kTile - 1) / kTile;
 }
 
-template <typename T, int D, int NT, int Warps, bool Whole>
-__global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attention_kernel(const AttentionPlan p) {
+template <typename T, int D, int NT, int Warps, AttendForm Form>
+__global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warps == 8 ? 1 : Warps == 4 ? 2 : 8) : attend_ctas(D)) attention_kernel(const AttentionPlan p) {
   using S = AttendShared<D, Warps>;
+  constexpr bool Whole = Form != AttendForm::kSplit, kCluster = Form == AttendForm::kCluster;
   constexpr int kAttendStages = S::kStages;
   constexpr int kAttendThreads = Warps * 32, kAttendTile = Warps * kAttendKeys;
   // The ring, then the merge's room (a whole unit's CTA merges in the ring).  Two
@@ -134,11 +139,11 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
   // set-up, then its tiles) --
   constexpr int kSetup = attend_setup(D);
   int row, off = 0, left = 1, length0;
-  const int ranks = Whole ? p.ranks : 1, rank = Whole ? static_cast<int>(blockIdx.x) : 0;
+    const int ranks = kCluster ? p.ranks : 1, rank = kCluster ? static_cast<int>(blockIdx.x) : 0;
   if constexpr (Whole) {
     row = blockIdx.z;
     length0 = row_length(p, row);
-    if (ranks > 1) cluster_arrive();   // every CTA of the cluster runs before its shared memory is written
+    if constexpr (kCluster) cluster_arrive();   // every CTA of the cluster runs before its shared memory is written
   } else {
     const int per = (a.rows + kAttendThreads - 1) / kAttendThreads;
     const int r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
@@ -411,12 +416,12 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
       }
     }
     __syncthreads();   // every warp is done with its products, and with the merge before this one
-    const bool whole = Whole ? ranks == 1 : t0 == 0 && count == n;
+    const bool whole = Whole ? !kCluster : t0 == 0 && count == n;
     // the cluster's inbox: [rank][head] (m, l), then [rank][join_each] four dimensions of O
     float2 *const inbox_ml = reinterpret_cast<float2 *>(words + Warps * 8);
     float4 *const inbox_o = reinterpret_cast<float4 *>(inbox_ml + kAttendRanks * NT * 8);
     const int join_each = Whole ? (heads * (D / 4) + ranks - 1) / ranks : 0;
-    if (Whole && !whole) cluster_wait();
+    if constexpr (kCluster) cluster_wait();
     const int64_t piece = 2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0);
     if (tid < (heads * Warps + 31) / 32 * 32) {   // whole warps: a lane per (head, warp)
       // the head's maximum and sum over the warps, each warp's factor, lse
@@ -433,7 +438,7 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
       if (live) {
         // a whole unit is divided here; no key with a weight gives zeros and log 0
         factor(w, h) = !whole ? f : sum == 0.f ? 0.f : f / sum;
-        if (Whole && !whole) {
+        if constexpr (kCluster) {
           for (int r = w; r < ranks; r += Warps) store_cluster(inbox_ml + rank * (NT * 8) + h, r, make_float2(top, sum));
         } else if (w == 0) {
           if (!whole) {
@@ -471,7 +476,7 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
         if (whole) {
           *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + row_now * a.out_stride + static_cast<int64_t>(head0 + nt * 8 + h) * D + c) =
               make_uint2(Element<T>::pack(o.x, o.y), Element<T>::pack(o.z, o.w));
-        } else if constexpr (Whole) {
+        } else if constexpr (kCluster) {
           const int to = (nt * (8 * D / 4) + i) / join_each;
           store_cluster(inbox_o + rank * join_each + (nt * (8 * D / 4) + i - to * join_each), to, o);
         } else {
@@ -479,7 +484,7 @@ __global__ void __launch_bounds__(Warps * 32, Whole ? 1 : attend_ctas(D)) attent
         }
       }
     }
-    if (Whole && !whole) {   // every CTA joins its slice of the heads' dimensions
+    if constexpr (kCluster) {   // every CTA joins its slice of the heads' dimensions
       cluster_arrive();
       cluster_wait();
       const int i = rank * join_each + tid, h = i / (D / 4), c = i % (D / 4) * 4;

@@ -4,6 +4,7 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <type_traits>
 
 #include "../../include/cruise_decoder.h"
 #include "decoder_attention.cuh"
@@ -131,17 +132,18 @@ cudaError_t rotate_typed(const RotateArgs &a, int device, cudaStream_t stream) {
 // unit as a cluster (0: the units are split over all CTAs).
 struct AttentionShape {
   int32_t groups, chunks, chunk, units;
+  int32_t warps;   // of a CTA that takes a unit, 0: units are split over all CTAs
   int32_t ranks;
   int grid;   // CTAs of the split form
 };
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int Warps, bool Cluster>
 cudaError_t allow_whole(int device, size_t *bytes) {
-  using Shared = AttendShared<D, kAttendWholeWarps>;
+  using Shared = AttendShared<D, Warps>;
   static_assert(Shared::kMergeBytes <= Shared::kRingBytes, "the merge takes the ring's room");
   static std::atomic<uint64_t> done{0};
-  *bytes = Shared::kRingBytes + kAttendWholeWarps * 32 + Shared::kInboxBytes(NT * 8);
-  return allow_shared(attention_kernel<T, D, NT, kAttendWholeWarps, true>, *bytes, device, done, true);
+  *bytes = Shared::kRingBytes + Warps * 32 + (Cluster ? Shared::kInboxBytes(NT * 8) : 0);
+  return allow_shared(attention_kernel<T, D, NT, Warps, Cluster ? AttendForm::kCluster : AttendForm::kWhole>, *bytes, device, done, Cluster);
 }
 
 // Clusters of `ranks` CTAs, an SM each, that run at once (the types' kernels do
@@ -158,10 +160,10 @@ int attention_fit(int ranks, int device) {
   DeviceScope scope(device);
   size_t shared = 0;
   int n = 0;
-  if (scope.error == cudaSuccess && allow_whole<__nv_bfloat16, D, NT>(device, &shared) == cudaSuccess) {
+  if (scope.error == cudaSuccess && allow_whole<__nv_bfloat16, D, NT, kAttendWholeWarps, true>(device, &shared) == cudaSuccess) {
     cudaLaunchAttribute attr{};
     const cudaLaunchConfig_t cfg = cluster_launch(dim3(ranks), kAttendWholeWarps * 32, shared, ranks, attr);
-    if (cudaOccupancyMaxActiveClusters(&n, attention_kernel<__nv_bfloat16, D, NT, kAttendWholeWarps, true>, &cfg) != cudaSuccess) n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, attention_kernel<__nv_bfloat16, D, NT, kAttendWholeWarps, AttendForm::kCluster>, &cfg) != cudaSuccess) n = 0;
   }
   if (n <= 0) {
     cudaGetLastError();
@@ -177,16 +179,48 @@ AttentionShape attention_shape(int32_t rows, int32_t nq, int32_t nkv, int32_t d,
   s.chunks = (s.groups + 15) / 16;
   s.chunk = (s.groups + s.chunks - 1) / s.chunks;
   s.units = nkv * s.chunks;
+  s.ranks = 1;
+  s.warps = 0;
+  s.grid = 0;
   const int sms = sm_count(device);
   const int64_t units = std::max<int64_t>(1, static_cast<int64_t>(rows) * s.units);
-  s.ranks = 0;
+  // Which form, in us for units x positions of head size 128 (28 heads over 4)
+  // where nothing else is said.  A CTA of one warp needs no merge and comes eight
+  // times to an SM, one of four twice, but each works through its unit alone:
+  //   8 x 16: one warp 2.6, four 2.8, eight 3.6; 8 x 64: 4.3, 2.8, 3.7
+  //   300 x 64: one 5.1, four 5.4; 300 x 128: 7.5, 6.4; 1200 x 256: 23.0, 28.6
+  //   (head size 64, whose four-warp CTAs are smaller: 600 x 128: 6.7, 5.7; 1200 x 128: 8.2, 9.3)
+  if (capacity <= kAttendKeys || (units * d >= 512 * capacity && capacity <= 512)) {
+    s.warps = 1;
+    return s;
+  }
   if (units <= sms) {
+    //   64 x 64: four 3.2, eight 3.6; 144 x 128: 4.4, 4.2
+    if (capacity <= 4 * kAttendKeys || (capacity <= 8 * kAttendKeys && 2 * units <= sms)) {
+      s.warps = 4;
+      return s;
+    }
+    // A cluster's join costs 1 us, the split's second kernel 4 and more, but the
+    // split also evens out lengths and uses every SM; a CTA takes 0.75 us per
+    // 128 positions.  16 x 256: one CTA 4.4, clusters of two 5.1; 32 x 384 of head size 64: 4.0, 4.6;
+    // 16 x 512: one 5.9, four 5.1; 16 x 2048: clusters 7.0, split 9.4; 4 x 8192: 8.0, 9.1;
+    // 4 x 16384: 12.2, 11.7; head size 64, 8 x 30000: 18.6, 16.4.
     const auto fit = d == 128 ? (s.chunk <= 8 ? attention_fit<128, 1> : attention_fit<128, 2>)
                               : (s.chunk <= 8 ? attention_fit<64, 1> : attention_fit<64, 2>);
-    const int64_t tiles = std::max<int64_t>(1, (capacity + kAttendWholeWarps * kAttendKeys - 1) / (kAttendWholeWarps * kAttendKeys));
-    int ranks = tiles <= 2 ? 1 : static_cast<int>(std::min<int64_t>({sms / units, tiles, kAttendRanks}));
+    constexpr int kTile = kAttendWholeWarps * kAttendKeys;
+    const int64_t tiles = (capacity + kTile - 1) / kTile;
+    int ranks = tiles <= 3 ? 1 : static_cast<int>(std::min<int64_t>({sms / units, tiles, kAttendRanks}));
     while (ranks > 1 && fit(ranks, device) < units) --ranks;
-    if (tiles <= 8 * ranks) s.ranks = ranks;
+    if (tiles <= 8 * ranks) {
+      s.warps = kAttendWholeWarps;
+      s.ranks = ranks;
+      return s;
+    }
+  } else if (capacity <= std::min<int64_t>(1024, 512 + units)) {
+    // 240 x 512: four warps a unit 13.6, split 18.9; 600 x 768: 46.2, 45.9; but the
+    // longest unit alone takes 15 ns a position: 240 rows of 1 to 1024: 13.9, split 11.1
+    s.warps = 4;
+    return s;
   }
   s.grid = sms * attend_ctas(d);
   return s;
@@ -218,13 +252,21 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
   p.slot_chunks = static_cast<uint32_t>(a.nkv * D / 8);
   p.scale_log2 = a.scale * 1.4426950408889634f;
   static std::atomic<uint64_t> done{0};
-  if (s.ranks > 0) {
+  if (s.warps > 0) {
     p.ranks = s.ranks;
-    size_t smem = 0;
-    const cudaError_t err = allow_whole<T, D, NT>(device, &smem);
-    if (err != cudaSuccess) return err;
-    return launch(attention_kernel<T, D, NT, kAttendWholeWarps, true>, dim3(s.ranks, s.units, a.rows), kAttendWholeWarps * 32, smem,
-                  s.ranks, stream, p);
+    const auto run = [&](auto warps, auto cluster) {
+      size_t smem = 0;
+      const cudaError_t err = allow_whole<T, D, NT, warps, cluster>(device, &smem);
+      if (err != cudaSuccess) return err;
+      return launch(attention_kernel<T, D, NT, warps, cluster ? AttendForm::kCluster : AttendForm::kWhole>, dim3(s.ranks, s.units, a.rows),
+                    warps * 32, smem, s.ranks, stream, p);
+    };
+    using Eight = std::integral_constant<int, kAttendWholeWarps>;
+    switch (s.warps) {
+      case 1: return run(std::integral_constant<int, 1>(), std::false_type());
+      case 4: return run(std::integral_constant<int, 4>(), std::false_type());
+      default: return s.ranks > 1 ? run(Eight(), std::true_type()) : run(Eight(), std::false_type());
+    }
   }
   p.by_unit = static_cast<int64_t>(a.rows) * s.units <= s.grid ? 1 : 0;
   size_t ml = 0, of = 0;
@@ -234,7 +276,7 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
   p.piece_ml = reinterpret_cast<float *>(w + ml);
   p.piece_of = reinterpret_cast<int4 *>(w + of);
   constexpr size_t smem = AttendShared<D, kAttendWarps>::kRingBytes + AttendShared<D, kAttendWarps>::kMergeBytes;
-  auto *kernel = attention_kernel<T, D, NT, kAttendWarps, false>;
+  auto *kernel = attention_kernel<T, D, NT, kAttendWarps, AttendForm::kSplit>;
   cudaError_t err = allow_shared(kernel, smem, device, done);
   if (err != cudaSuccess) return err;
   err = launch(kernel, dim3(s.grid), kAttendWarps * 32, smem, 1, stream, p);
@@ -360,7 +402,7 @@ cudaError_t launch_rotate_store(const RotateArgs &a, int device, cudaStream_t st
 
 int64_t attention_workspace(int32_t rows, int32_t nq, int32_t nkv, int32_t d, int64_t capacity, int device) {
   const AttentionShape s = attention_shape(rows, nq, nkv, d, capacity, device);
-  if (s.ranks > 0) return 0;
+  if (s.warps > 0) return 0;
   return static_cast<int64_t>(pieces_bytes(s.grid, s.chunk <= 8 ? 8 : 16, d, nullptr, nullptr));
 }
 

@@ -196,6 +196,10 @@ def check_attend(case, **keep):
     ([256, 257, 300], 16, 1, 128, 16, None),
     ([16384, 5], 8, 1, 128, 128, None),
     ([1024] * 36 + [0], 28, 4, 128, 128, None),     # one CTA for each unit, and for each SM
+    ([16, 3, 0, 1], 14, 2, 128, 16, 1),             # a warp for each unit
+    ([1, 100, 33, 0, 17] * 40, 16, 4, 64, 16, 8),   # (more of them than run at once)
+    ([31, 64, 1, 0], 24, 2, 64, 16, 4),             # four warps for each unit
+    ([200, 500, 0, 1, 64, 65] * 30, 11, 1, 128, 24, None),
     ([513, 0, 1, 2000, 64, 5000], 7, 1, 128, 16, 2000),         # wide tables: units split over all CTAs
     ([3000, 1, 0, 777], 32, 8, 64, 24, 1000),
     ([1025] * 5, 16, 1, 64, 32, 600),
