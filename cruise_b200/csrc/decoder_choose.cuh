@@ -11,7 +11,7 @@
 //
 // A cluster of CTAs shares a row, a slice of the vocabulary each; the slices'
 // maxima meet in the first CTA's shared memory, so a call is one launch and
-// keeps no state.  Few tokens of a slice are in the history or the bias list.  Four
+// keeps no state.  Few tokens of a slice are in the history or the bias list.  Four or eight
 // warps deal with them: a bit map in shared memory marks them, their rank in it
 // is their place in a table of occurrences, and from that come their processed
 // values.  Meanwhile the other warps stream over the slice and know nothing of
@@ -31,8 +31,8 @@ namespace cruise {
 namespace ops {
 
 constexpr int kChooseThreads = 512;
-constexpr int kChooseTableThreads = 128;   // of them, those of the marked tokens
-constexpr int kChooseStreamThreads = kChooseThreads - kChooseTableThreads;
+constexpr int kChooseFewThreads = 128;     // of them, those of the marked tokens,
+constexpr int kChooseManyThreads = 256;    // and where these are many for the slice
 constexpr int kChooseCtas = 2;             // CTAs per SM
 constexpr int kChooseMaxCluster = 16;
 constexpr int kChooseAhead = 4;            // vectors a thread has in flight
@@ -120,15 +120,17 @@ struct Logit<__nv_bfloat16> : LogitHalf<__nv_bfloat16> {};
 template <>
 struct Logit<__half> : LogitHalf<__half> {};
 
-template <typename T>
+template <typename T, int Table>
 __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(const ChooseArgs a, const int32_t slice) {
   extern __shared__ __align__(16) uint32_t shared[];
+  constexpr int kStream = kChooseThreads - Table;   // threads of the stream
   __shared__ ChooseBest warp_part[kChooseThreads / 32];
   __shared__ ChooseBest parts[kChooseMaxCluster];
-  __shared__ int32_t scan[kChooseTableThreads / 32];
+  __shared__ int32_t scan[Table / 32];
+  __shared__ uint32_t spare[32];      // where entries of other slices leave what they would mark
   __shared__ int32_t shared_listed;   // marked tokens of the slice
   __shared__ int32_t retakes;         // stream threads whose maximum is one of them
-  __shared__ uint16_t retake_list[kChooseStreamThreads];
+  __shared__ uint16_t retake_list[kStream];
   constexpr int kVec = Logit<T>::kVec;
   const int tid = threadIdx.x, row = blockIdx.y, ctas = gridDim.x;
   const int part = ctas > 1 ? static_cast<int>(cluster_rank()) : 0;
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
   const int32_t lead = min(width, static_cast<int32_t>(((16 - (reinterpret_cast<uintptr_t>(logits) & 15)) & 15) / sizeof(T)));
   const int32_t vectors = (width - lead) / kVec;
   const int32_t rest = lead + vectors * kVec;
-  const int32_t steps = (vectors + kChooseStreamThreads - 1) / kChooseStreamThreads;
+  const int32_t steps = (vectors + kStream - 1) / kStream;
   const int32_t last_word = (width - 1) >> 5;
   const bool split = lead % kVec != 0;   // a vector's mask bits may go on in the next word
   const uint4 *const stream = reinterpret_cast<const uint4 *>(logits + lead);
@@ -163,7 +165,7 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
   int32_t top_at = -1;
   if (tid == 0) retakes = 0;
 
-  if (active && tid < kChooseTableThreads) {
+  if (active && tid < Table) {
     // -- the marked tokens.  What a thread does for an entry it does without
     // branches (an entry of another slice marks nothing and counts nothing), so
     // that a batch's entries overlap; the first history entries are fetched with
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
     auto fetch = [&](int32_t i0, int32_t end) {
 #pragma unroll
       for (int k = 0; k < kChooseBatch; ++k) {
-        const int32_t i = i0 + k * kChooseTableThreads;
+        const int32_t i = i0 + k * Table;
         id[k] = i < end ? history[i] : -1;
       }
     };
@@ -192,33 +194,33 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
     if (a.frequency != nullptr) freq = a.frequency[row];
     if (a.presence != nullptr) pres = a.presence[row];
     const int32_t counted = rep != 1.f || freq != 0.f || pres != 0.f ? min(max(length, 0), history_width) : 0;
-    constexpr int32_t kStride = kChooseBatch * kChooseTableThreads;
+    constexpr int32_t kStride = kChooseBatch * Table;
     int32_t listed = 0;
     if (counted + biases > 0) {
       // a vocabulary id as a token of this slice; others are at least `width`
       auto here = [&](int32_t v) { return static_cast<uint32_t>(v) - static_cast<uint32_t>(v0); };
       auto mark = [&](uint32_t n) { atomicOr(&marks[n >> 5], 1u << (n & 31)); };
       auto rank = [&](uint32_t n) { return ranks[n >> 5] + __popc(marks[n >> 5] & ((1u << (n & 31)) - 1)); };
-      for (int32_t i = tid; i < words / 4; i += kChooseTableThreads) reinterpret_cast<uint4 *>(marks)[i] = make_uint4(0, 0, 0, 0);
+      for (int32_t i = tid; i < words / 4; i += Table) reinterpret_cast<uint4 *>(marks)[i] = make_uint4(0, 0, 0, 0);
       const int32_t most = min(counted + biases, width);
-      for (int32_t i = tid; i < most; i += kChooseTableThreads) counts[i] = 0;
-      named_sync(1, kChooseTableThreads);
+      for (int32_t i = tid; i < most; i += Table) counts[i] = 0;
+      named_sync(1, Table);
       for (int32_t i0 = tid; i0 - tid < counted; i0 += kStride) {
         if (i0 != tid) fetch(i0, counted);
 #pragma unroll
         for (int k = 0; k < kChooseBatch; ++k) {
-          if (i0 - tid + k * kChooseTableThreads >= counted) break;   // uniform: short histories run little code
+          if (i0 - tid + k * Table >= counted) break;   // uniform: short histories run little code
           const uint32_t n = here(id[k]);
-          const bool mine = i0 + k * kChooseTableThreads < counted && n < static_cast<uint32_t>(width);
-          atomicOr(&marks[mine ? n >> 5 : 0], mine ? 1u << (n & 31) : 0u);
+          const bool mine = i0 + k * Table < counted && n < static_cast<uint32_t>(width);
+          atomicOr(mine ? &marks[n >> 5] : &spare[tid & 31], mine ? 1u << (n & 31) : 0u);
         }
       }
       if (here(bias_id) < static_cast<uint32_t>(width) && tid < biases) mark(here(bias_id));
-      for (int32_t i = tid + kChooseTableThreads; i < biases; i += kChooseTableThreads)
+      for (int32_t i = tid + Table; i < biases; i += Table)
         if (here(bias_token[i]) < static_cast<uint32_t>(width)) mark(here(bias_token[i]));
-      named_sync(1, kChooseTableThreads);
+      named_sync(1, Table);
       // ranks: every thread its run of words
-      const int32_t per = (words / 4 + kChooseTableThreads - 1) / kChooseTableThreads * 4;
+      const int32_t per = (words / 4 + Table - 1) / Table * 4;
       const int32_t w0 = min(tid * per, words), w1 = min(w0 + per, words);
       int32_t mine = 0;
       for (int32_t w = w0; w < w1; w += 4) {
@@ -232,9 +234,9 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
         if ((tid & 31) >= o) incl += v;
       }
       if ((tid & 31) == 31) scan[tid >> 5] = incl;
-      named_sync(1, kChooseTableThreads);
+      named_sync(1, Table);
 #pragma unroll
-      for (int w = 0; w < kChooseTableThreads / 32; ++w) {
+      for (int w = 0; w < Table / 32; ++w) {
         if (w < (tid >> 5)) incl += scan[w];
         listed += scan[w];
       }
@@ -245,18 +247,19 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
         *reinterpret_cast<uint4 *>(ranks + w) = make_uint4(at, b, c, d);
         at = d + __popc(m.w);
       }
-      named_sync(1, kChooseTableThreads);
+      named_sync(1, Table);
       for (int32_t i0 = tid; i0 - tid < counted; i0 += kStride) {
         if (counted > kStride) fetch(i0, counted);
 #pragma unroll
         for (int k = 0; k < kChooseBatch; ++k) {
-          if (i0 - tid + k * kChooseTableThreads >= counted) break;
-          const int32_t i = i0 + k * kChooseTableThreads;
+          if (i0 - tid + k * Table >= counted) break;
+          const int32_t i = i0 + k * Table;
           const bool mine = i < counted && here(id[k]) < static_cast<uint32_t>(width);
           const uint32_t n = mine ? here(id[k]) : 0, r = mine ? rank(n) : 0;   // (slot 0 exists)
           if (mine) list[r] = n;   // the token's entries agree
-          atomicOr(&counts[r], mine && i < prompt ? kInPrompt : 0u);
-          atomicAdd(&counts[r], mine && i >= prompt ? 1u : 0u);
+          uint32_t *const count = mine ? &counts[r] : &spare[tid & 31];
+          atomicOr(count, i < prompt ? kInPrompt : 0u);
+          atomicAdd(count, i >= prompt ? 1u : 0u);
         }
       }
       auto mark_bias = [&](uint32_t n) {
@@ -267,8 +270,8 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
         }
       };
       if (tid < biases) mark_bias(here(bias_id));
-      for (int32_t i = tid + kChooseTableThreads; i < biases; i += kChooseTableThreads) mark_bias(here(bias_token[i]));
-      named_sync(1, kChooseTableThreads);
+      for (int32_t i = tid + Table; i < biases; i += Table) mark_bias(here(bias_token[i]));
+      named_sync(1, Table);
       // the processed value takes the place of the occurrences
       auto rules = [&](uint32_t n, uint32_t r, float x) {
         const uint32_t word = counts[r], times = word & kCount;
@@ -284,20 +287,20 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
       };
       // (in place, the stream may have masked a logit already: -inf then, as here)
       constexpr int kTogether = 4;
-      for (int32_t i0 = tid; i0 < listed; i0 += kTogether * kChooseTableThreads) {
+      for (int32_t i0 = tid; i0 < listed; i0 += kTogether * Table) {
         T raw[kTogether];
 #pragma unroll
-        for (int k = 0; k < kTogether; ++k) raw[k] = logits[list[min(i0 + k * kChooseTableThreads, listed - 1)]];
+        for (int k = 0; k < kTogether; ++k) raw[k] = logits[list[min(i0 + k * Table, listed - 1)]];
 #pragma unroll 1
-        for (int k = 0; k < kTogether && i0 - tid + k * kChooseTableThreads < listed; ++k) {
-          const int32_t i = i0 + k * kChooseTableThreads;
+        for (int k = 0; k < kTogether && i0 - tid + k * Table < listed; ++k) {
+          const int32_t i = i0 + k * Table;
           if (i < listed && (counts[i] & kHasBias) == 0) rules(list[i], i, Logit<T>::one(&raw[0]));
 #pragma unroll
           for (int q = 0; q + 1 < kTogether; ++q) raw[q] = raw[q + 1];
         }
       }
-      if (biases > 0) named_sync(1, kChooseTableThreads);
-      for (int32_t i = tid; i < biases; i += kChooseTableThreads) {   // entries of one token add up
+      if (biases > 0) named_sync(1, Table);
+      for (int32_t i = tid; i < biases; i += Table) {   // entries of one token add up
         const int32_t v = bias_token[i];
         const uint32_t n = here(v);
         if (n >= static_cast<uint32_t>(width) || (i > 0 && bias_token[i - 1] == v)) continue;
@@ -310,7 +313,7 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
     if (tid == 0) shared_listed = listed;
   } else if (active) {
     // -- the stream: every token as if the rules left it --
-    const int32_t me = tid - kChooseTableThreads;
+    const int32_t me = tid - Table;
     float worst = -INFINITY;   // NaN and +inf stay in it: no rule makes them finite
     if (vectors > 0) {
       uint4 ahead[kChooseAhead];
@@ -320,7 +323,7 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
         // Nothing here waits for a load; a step past the end fetches the slice's last
         // vector again, for a load under a condition would be waited for.
         auto fetch = [&](int k, int32_t step) {
-          const int32_t i = min(step * kChooseStreamThreads + me, vectors - 1);
+          const int32_t i = min(step * kStream + me, vectors - 1);
           ahead[k] = stream[i];
           if (kMask) {
             const int32_t w = (lead + i * kVec) >> 5;
@@ -335,7 +338,7 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
         for (int32_t step0 = 0; step0 < steps; step0 += kChooseAhead) {
 #pragma unroll
           for (int k = 0; k < kChooseAhead; ++k) {
-            const int32_t step = step0 + k, vector = step * kChooseStreamThreads + me;
+            const int32_t step = step0 + k, vector = step * kStream + me;
             float x[kVec];
             Logit<T>::unpack(ahead[k], x);
             if (kMask) masked(x, split ? __funnelshift_r(open[k], open_next[k], shift) : open[k] >> shift);
@@ -368,7 +371,7 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
       };
       using Yes = std::true_type;
       using No = std::false_type;
-      static_assert(kChooseStreamThreads * kVec % 32 == 0, "a step is a whole number of mask words");
+      static_assert(kStream * kVec % 32 == 0, "a step is a whole number of mask words");
       if (allowed != nullptr)
         out != nullptr ? run(Yes{}, Yes{}) : run(Yes{}, No{});
       else
@@ -407,7 +410,7 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
     const bool retake = top_at >= 0 && ruled(top_at);
     if (retake) {
       top = -INFINITY;
-      retake_list[atomicAdd(&retakes, 1)] = static_cast<uint16_t>(tid - kChooseTableThreads);
+      retake_list[atomicAdd(&retakes, 1)] = static_cast<uint16_t>(tid - Table);
     }
     if (__syncthreads_or(retake)) {
       const int32_t again = retakes;
@@ -416,12 +419,12 @@ __global__ void __launch_bounds__(kChooseThreads, kChooseCtas) choose_kernel(con
         for (int32_t q = tid >> 5; q < again; q += kWarps) {
           float value = -INFINITY;
           int32_t at = 0;
-          for (int32_t vector = (tid & 31) * kChooseStreamThreads + retake_list[q]; vector < vectors; vector += 32 * kChooseStreamThreads)
+          for (int32_t vector = (tid & 31) * kStream + retake_list[q]; vector < vectors; vector += 32 * kStream)
             look(vector, value, at);
           if (value > -INFINITY) better(best, value, v0 + at);
         }
       } else if (retake) {
-        for (int32_t vector = tid - kChooseTableThreads; vector < vectors; vector += kChooseStreamThreads) look(vector, top, top_at);
+        for (int32_t vector = tid - Table; vector < vectors; vector += kStream) look(vector, top, top_at);
       }
     }
     if (top > -INFINITY) better(best, top, v0 + top_at);

@@ -312,7 +312,7 @@ int choose_fit(int log, bool alone, int device) {
   cudaLaunchAttribute attr{};
   const cudaLaunchConfig_t cfg = cluster_launch(dim3(ctas), kChooseThreads, alone ? kChooseAlone : kChooseAlone / 2, ctas, attr);
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, choose_kernel<T>, &cfg) != cudaSuccess || n <= 0) {
+  if (cudaOccupancyMaxActiveClusters(&n, choose_kernel<T, kChooseFewThreads>, &cfg) != cudaSuccess || n <= 0) {
     cudaGetLastError();
     return 1;
   }
@@ -322,8 +322,9 @@ int choose_fit(int log, bool alone, int device) {
 
 template <typename T>
 cudaError_t choose_typed(const ChooseArgs &a, int device, cudaStream_t stream) {
-  static std::atomic<uint64_t> done{0};
-  cudaError_t err = allow_shared(choose_kernel<T>, kChooseShared, device, done, true);
+  static std::atomic<uint64_t> done{0}, done_many{0};
+  cudaError_t err = allow_shared(choose_kernel<T, kChooseFewThreads>, kChooseShared, device, done, true);
+  if (err == cudaSuccess) err = allow_shared(choose_kernel<T, kChooseManyThreads>, kChooseShared, device, done_many, true);
   if (err != cudaSuccess) return err;
   const int64_t entries = (a.history != nullptr ? a.history_width : 0) + static_cast<int64_t>(a.bias_token != nullptr ? a.bias_width : 0);
   // CTAs per row: a CTA takes about 5 us for the chain of its steps and the
@@ -354,7 +355,13 @@ cudaError_t choose_typed(const ChooseArgs &a, int device, cudaStream_t stream) {
   // memory: a successor's CTAs, which come while this launch drains, would else
   // settle two on the SMs it left idle (64 rows of 50257: 10.9 us, 8.8 so)
   const size_t shared = choose_shared(slice, entries);
-  return launch(choose_kernel<T>, dim3(ctas, a.rows), kChooseThreads, alone ? std::max(shared, kChooseAlone) : shared, ctas,
+  // The marked tokens and the stream share a CTA's threads: 100 rows of 32000 with
+  // 1000 entries 8.0 us with few threads for the former and 6.9 with many, with 30
+  // entries and processed logits 7.8 and 9.4; 100 rows of 64000: 9.9 and 13.6,
+  // with 4000 entries 17.9 and 13.8; 256 rows of 152064 with 4000: 33 and 41.
+  const double streamed = slice * (sizeof(T) / 4.0) * (a.processed != nullptr ? 2 : 1);
+  auto *kernel = 36.0 * entries >= streamed ? choose_kernel<T, kChooseManyThreads> : choose_kernel<T, kChooseFewThreads>;
+  return launch(kernel, dim3(ctas, a.rows), kChooseThreads, alone ? std::max(shared, kChooseAlone) : shared, ctas,
                 stream, a, slice);
 }
 
