@@ -141,7 +141,9 @@ __global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warp
   int row, off = 0, left = 1, length0;
     const int ranks = kCluster ? p.ranks : 1, rank = kCluster ? static_cast<int>(blockIdx.x) : 0;
   if constexpr (Whole) {
-    row = blockIdx.z;
+    // grid: (CTAs of the cluster, units, rows), or (units, rows in y and z)
+    row = kCluster ? blockIdx.z : blockIdx.z * gridDim.y + blockIdx.y;
+    if (row >= a.rows) return;
     length0 = row_length(p, row);
     if constexpr (kCluster) cluster_arrive();   // every CTA of the cluster runs before its shared memory is written
   } else {
@@ -214,7 +216,7 @@ __global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warp
       s.length = c.length;
       s.n = row_tiles<Warps>(s.length);
       if constexpr (Whole) {
-        s.unit = blockIdx.y;
+        s.unit = kCluster ? blockIdx.y : blockIdx.x;
         s.t0 = rank;   // and every `ranks`-th tile from there, so that the first is known before the length
         s.count = s.n > rank ? (s.n - rank + ranks - 1) / ranks : 0;
         c.left = 0;

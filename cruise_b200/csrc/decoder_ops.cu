@@ -258,8 +258,10 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
       size_t smem = 0;
       const cudaError_t err = allow_whole<T, D, NT, warps, cluster>(device, &smem);
       if (err != cudaSuccess) return err;
-      return launch(attention_kernel<T, D, NT, warps, cluster ? AttendForm::kCluster : AttendForm::kWhole>, dim3(s.ranks, s.units, a.rows),
-                    warps * 32, smem, s.ranks, stream, p);
+      const unsigned units = s.units, rows = a.rows, most = 65535;
+      const dim3 grid = cluster ? dim3(s.ranks, units, rows) : dim3(units, std::min(rows, most), (rows + most - 1) / most);
+      return launch(attention_kernel<T, D, NT, warps, cluster ? AttendForm::kCluster : AttendForm::kWhole>, grid, warps * 32, smem,
+                    s.ranks, stream, p);
     };
     using Eight = std::integral_constant<int, kAttendWholeWarps>;
     switch (s.warps) {

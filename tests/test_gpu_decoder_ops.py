@@ -318,6 +318,24 @@ def test_paged_attention_lse_joins_parts():
     assert float(((joined - want).abs() - (3 * bound + 2 * lse_bound[..., None] + 2.0 ** -8 * want.abs().amax())).max()) <= 0
 
 
+@pytest.mark.parametrize("width", [1, 4, 40])
+def test_paged_attention_of_very_many_rows(width):
+    """More rows than a grid's second dimension, sharing a few blocks (40 blocks of
+    16 a row: split over all CTAs)."""
+    from cruise_b200.decoder_ops import paged_attention
+
+    g = gen(12)
+    rows = 140001
+    key, value = (randn(g, 9, 16, 1, 64, dtype=BF16) for _ in range(2))
+    table = torch.randint(-1, 10, (rows, width), device="cuda", dtype=torch.int32, generator=g)
+    lens = torch.randint(0, 33, (rows,), device="cuda", dtype=torch.int32, generator=g)
+    q = randn(g, rows, 2, 64, dtype=BF16)
+    out = paged_attention(q, key, value, table, lens)
+    some = torch.cat([torch.arange(40), torch.arange(65520, 65560), torch.arange(131060, 131080), torch.arange(rows - 40, rows)]).cuda()
+    want, _, bound, _ = attention_reference(q[some], key, value, table[some], lens[some])
+    within(out[some], want, bound, "out")
+
+
 def test_paged_attention_without_rows_or_columns():
     from cruise_b200.decoder_ops import paged_attention
 
