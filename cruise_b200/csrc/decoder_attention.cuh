@@ -12,6 +12,26 @@
 // the columns, so a group of up to 8 heads reads its keys once.  Probabilities
 // are rounded to the cache's type for the second product (relative 2^-9 in
 // bf16, 2^-12 in fp16, as the values they weight); m, l and O are fp32.
+//
+// What bounds it is the cache's bytes: a key and its value, 4 d bytes, take 4 d
+// operations for each of the group's heads, far below the tensor pipe (8% of
+// its cycles at 64 ragged rows).  So the products are the warp-wide ones, whose
+// operands a warp takes from its own ring as they arrive, 16 keys a step, with
+// no barrier between warps until the unit's end; larger tiles would only wait
+// for more bytes.  256 rows of up to 4096 (28 heads over 4 of 128) take 212 us,
+// 98% of the copy bandwidth; one row of 131071 47 us (87%: 3 us to start, 3 for
+// the join); 64 ragged rows of up to 16384 in pages of 16, head size 64, 46 us
+// (75%: units of a few steps, and two steps of copies in flight per warp).  Few
+// and short units are bounded by the chain of start, first loads, products and
+// merge: 4 rows of 256 4.3 us, 4 of 16 2.6.
+//
+// Which CTAs take a unit (a row and a KV head, at most 16 query heads):
+//   split:   all CTAs share all tiles evenly, whatever the rows' lengths, and a
+//            second kernel joins the pieces of the units that were cut;
+//   whole:   a CTA of one, four or eight warps takes a unit;
+//   cluster: up to 16 CTAs of eight warps take a unit, every n-th tile each,
+//            and join over their shared memory.
+// The launch chooses by rows, units and capacity, and has the times.
 #pragma once
 
 #include "decoder_common.cuh"
@@ -28,11 +48,14 @@ constexpr int kJoinThreads = 512;
 constexpr int kJoinBatch = 6;        // pieces a thread has in flight
 
 // CTAs per SM that share the work: what shared memory (head size 128) or
-// registers (64, for 16 heads a unit) allow.
+// registers (64, for 16 heads a unit) allow.  (64 ragged rows of head size 64:
+// 45.8 us with three, 59.1 with four.)
 __host__ __device__ constexpr int attend_ctas(int d) { return d == 128 ? 2 : 3; }
 
 // What starting a unit costs, in tiles: the pipeline fills and the warps' parts
-// meet once per unit, whatever its length.
+// meet once per unit, whatever its length.  (Shares of tiles alone: 64 ragged rows
+// 68 us instead of 46, 128 rows of 100 to 500 23.9 instead of 21.3.)  A share is at
+// least one tile and its setup: with two setups 22 rows of 1576 took 12.1 us, not 10.9.
 __host__ __device__ constexpr int attend_setup(int d) { return d == 128 ? 2 : 4; }
 
 // Pieces of split units: CTA c leaves its first piece (of a unit that began
@@ -63,7 +86,11 @@ enum class AttendForm { kSplit, kWhole, kCluster };
 
 template <int D, int Warps>
 struct AttendShared {
-  static constexpr int kStages = Warps == kAttendWholeWarps && D == 64 ? 6 : 3;   // steps of a warp's ring
+  // Steps of a warp's ring.  Two steps of copies in flight keep an SM's copy path
+  // busy with 8 warps of head size 128, or 12 of 64; with one (two stages) 64 ragged
+  // rows took 52.7 us, not 45.8.  Eight warps of head size 64 have room for five: 4 rows
+  // x 8 heads of 3000 7.9 us, with two 9.4.
+  static constexpr int kStages = Warps == kAttendWholeWarps && D == 64 ? 6 : 3;
   static constexpr int kRowBytes = D * 2;
   static constexpr int kStageBytes = 2 * kAttendKeys * kRowBytes;   // K then V
   static constexpr int kRingBytes = Warps * kStages * kStageBytes;
@@ -125,7 +152,7 @@ __global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warp
   __shared__ float merge_f_room[NT == 1 ? Warps * 8 : 1];   // (16 heads: the factor replaces the maximum)
   auto factor = [&](int w, int h) -> float & { return NT == 1 ? merge_f_room[w * 8 + h] : merge_ml[w][h][0]; };
   uint32_t *const words = reinterpret_cast<uint32_t *>(ring + S::kRingBytes);
-  auto word = [&](int line, int i) -> uint32_t & {   // word i < 4 of 8 * Warps lines
+  auto word = [&](int line, int i) -> uint32_t & {   // word i < 4 (8) of 8 * Warps lines
     return Whole ? words[line * 8 + i] : words[line * S::kMergeStride + D + i];
   };
   static_assert(kAttendStages <= (Whole ? 8 : 4), "a line holds a warp's masks");
@@ -528,7 +555,9 @@ __global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warp
 
 // Joins the pieces of a split unit (piece_of), `heads_each` of its heads a CTA.
 // D / 4 lanes take a head's row of a piece, four dimensions each; the lanes'
-// groups share the heads and their pieces.
+// groups share the heads and their pieces.  The pieces come from L2 and latency
+// bounds it: 3 us of 47 for one row of 131071 (4 units of 74 pieces, a CTA for
+// each of their heads; with a CTA for each unit 52 us in all).
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kJoinThreads, 1) attention_join_kernel(const AttentionPlan p, const int32_t heads_each) {
   constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;

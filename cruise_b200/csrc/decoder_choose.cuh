@@ -19,6 +19,15 @@
 // element.  After the barrier between the two, a thread whose maximum is a marked
 // token has its elements gone over again without them, by a warp together, and
 // the marked tokens' values are written over the stream's.
+//
+// What bounds it: for many rows the logits' bytes.  256 rows of 152064 with every
+// rule and the processed logits written take 74 us, 66% of the copy bandwidth (the
+// stream alone 57; then the marked tokens' values and second looks, while little
+// is in flight).  For few rows the chain of the marked tokens' steps (clear, mark,
+// rank, count, value, compare): 4.1 us for one row of 4096, 5.5 for 4 of 152064,
+// 8.0 for 64 of 50257 with 1000 entries each.  Two kernels, one for the marked
+// tokens, took 126 us for the 256 rows; one CTA's warps doing first the one and
+// then the other 82.
 #pragma once
 
 #include <climits>
@@ -35,8 +44,8 @@ constexpr int kChooseFewThreads = 128;     // of them, those of the marked token
 constexpr int kChooseManyThreads = 256;    // and where these are many for the slice
 constexpr int kChooseCtas = 2;             // CTAs per SM
 constexpr int kChooseMaxCluster = 16;
-constexpr int kChooseAhead = 4;            // vectors a thread has in flight
-constexpr int kChooseBatch = 8;            // history entries a thread has in flight
+constexpr int kChooseAhead = 4;            // vectors a thread has in flight (256 rows of 152064: 74 us; two 78, six 79)
+constexpr int kChooseBatch = 8;            // history entries a thread has in flight (four: 78)
 constexpr size_t kChooseShared = 200 * 1024;
 constexpr size_t kChooseAlone = 118 * 1024;   // shared memory that leaves an SM no second CTA
 constexpr int32_t kChooseMaxVocab = 1 << 20;

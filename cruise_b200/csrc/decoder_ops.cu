@@ -70,8 +70,9 @@ cudaError_t allow_shared(Kernel kernel, size_t bytes, int device, std::atomic<ui
 }
 
 // Launches a kernel so that it may come onto the SMs while its predecessor in
-// the stream drains; it waits for that inside (follow_predecessor).  `cluster`
-// CTAs of x share their shared memory.
+// the stream drains; it waits for that inside (follow_predecessor): calls of 4 rows
+// of 256 one after the other take 4.8 us each so, 6.3 without.  `cluster` CTAs of x
+// share their shared memory.
 template <typename... Params, typename... Actual>
 cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, size_t shared, int cluster, cudaStream_t stream,
                    const Actual &...args) {
@@ -114,7 +115,8 @@ cudaError_t rotate_typed(const RotateArgs &a, int device, cudaStream_t stream) {
   constexpr int kHeads = 512 / D;   // heads of a kind a warp moves per round
   const int all = (a.nq + kHeads - 1) / kHeads + 2 * ((a.nkv + kHeads - 1) / kHeads);
   // as many rounds per warp as still leave 16 warps per SM: few tokens spread
-  // their heads over the GPU, many keep their table row in registers
+  // their heads over the GPU, many keep their table row in registers (4 tokens: 2.1 us
+  // with one round, 4.1 with all; 8192 tokens: 65 and 31)
   const int64_t want = static_cast<int64_t>(sm_count(device)) * 16;
   const int rounds = static_cast<int>(std::clamp<int64_t>(static_cast<int64_t>(a.tokens) * all / want, 1, all));
   const int warps_per_token = (all + rounds - 1) / rounds;
@@ -270,6 +272,8 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
       default: return s.ranks > 1 ? run(Eight(), std::true_type()) : run(Eight(), std::false_type());
     }
   }
+  // where the join looks: at every unit while they are no more than the CTAs (one
+  // row of 131071: 47 us; a join per CTA, most with nothing to do, 51)
   p.by_unit = static_cast<int64_t>(a.rows) * s.units <= s.grid ? 1 : 0;
   size_t ml = 0, of = 0;
   pieces_bytes(s.grid, NT * 8, D, &ml, &of);
@@ -284,6 +288,7 @@ cudaError_t attention_typed(const AttentionArgs &a, const AttentionShape &s, int
   err = launch(kernel, dim3(s.grid), kAttendWarps * 32, smem, 1, stream, p);
   if (err != cudaSuccess) return err;
   // few units: a CTA for some heads of each, so that the join is spread over the SMs
+  // (one row of 131071: 47.1 us, 52.0 with all heads of a unit in one)
   const int64_t units = static_cast<int64_t>(a.rows) * s.units;
   const int entries = p.by_unit ? static_cast<int>(units) : s.grid;
   const int each = std::clamp((s.chunk * entries + sm_count(device) - 1) / sm_count(device), 1, s.chunk);
@@ -332,8 +337,8 @@ cudaError_t choose_typed(const ChooseArgs &a, int device, cudaStream_t stream) {
   // CTAs per row: a CTA takes about 5 us for the chain of its steps and the
   // marked tokens (as long as it streams 32768 fp32 logits), clusters 1 us more;
   // two to an SM, the first takes 1.3 and the stream 1.6 times as long.  One row
-  // of 152064: 6.9 us with 16 CTAs, 12 with one; 17 rows: 8.2 with 4; 64 rows:
-  // 17 with 2, 26 with one.
+  // of 152064 with 1000 entries: 6.0 us with 16 CTAs, 7.6 with four, 14.3 with one;
+  // 17 rows: 12.9, 8.0, 16.3; 64 rows: 36 with 16, 12.6 with four, 26 with one.
   int best = 0;
   bool alone = false;
   double least = 0;
@@ -355,7 +360,7 @@ cudaError_t choose_typed(const ChooseArgs &a, int device, cudaStream_t stream) {
   const int32_t slice = choose_slice(a.vocab, ctas);
   // Where every CTA can have an SM of its own it takes more than half its shared
   // memory: a successor's CTAs, which come while this launch drains, would else
-  // settle two on the SMs it left idle (64 rows of 50257: 10.9 us, 8.8 so)
+  // settle two on the SMs it left idle (64 rows of 50257: 11.2 us, 8.0 so)
   const size_t shared = choose_shared(slice, entries);
   // The marked tokens and the stream share a CTA's threads: 100 rows of 32000 with
   // 1000 entries 8.0 us with few threads for the former and 6.9 with many, with 30
