@@ -20,8 +20,8 @@
 namespace cruise {
 namespace ops {
 
-// 8192 tokens: 31.0 us with five CTAs per SM, 35.2 with four (six leave too few
-// registers for the factors); 31.0 with three rounds of loads in flight, 35.9 with two.
+// 8192 tokens: 31.0 us with five CTAs per SM, 35.2 with four (six would leave 85
+// registers for the 96 in use); 31.0 with three rounds of loads in flight, 35.9 with two.
 constexpr int kRotateThreads = 128;
 constexpr int kRotateCtas = 5;    // CTAs per SM
 constexpr int kRotateBatch = 3;
