@@ -499,9 +499,10 @@ static int32_t check_attention_sizes(const char *op, int32_t rows, int32_t num_h
     return refuse("%s: %d rows of %d query heads over %d KV heads (a multiple, at most 1024)", op, rows, num_heads, num_kv_heads);
   if (head_dim != 64 && head_dim != 128) return refuse("%s: head size %d (64 or 128)", op, head_dim);
   constexpr int kTile = kAttendWarps * kAttendKeys;
-  if (capacity < 0 || capacity > kMaxIndex - kTile) return refuse("%s: a capacity of %lld positions (below 2^31)", op, static_cast<long long>(capacity));
+  // (the kernels count positions a few tiles past the end, and work up to a CTA's share past it, in 32 bits)
+  if (capacity < 0 || capacity > kMaxIndex - 4 * kTile) return refuse("%s: a capacity of %lld positions (below 2^31)", op, static_cast<long long>(capacity));
   const int64_t units = static_cast<int64_t>(num_kv_heads) * ((num_heads / num_kv_heads + 15) / 16);
-  if (rows * units * (std::max<int64_t>(1, (capacity + kTile - 1) / kTile) + attend_setup(head_dim)) > kMaxIndex)
+  if (rows * units * (std::max<int64_t>(1, (capacity + kTile - 1) / kTile) + attend_setup(head_dim)) > kMaxIndex - 1024)
     return refuse("%s: rows x KV heads x capacity / %d passes 2^31", op, kTile);
   return 0;
 }
@@ -584,7 +585,8 @@ int32_t cruise_decoder_choose(const void *logits, int64_t logits_stride, int32_t
   if (rows < 0 || rows > 65535 || vocab < 1 || vocab > kChooseMaxVocab)
     return refuse("%s: %d rows of %d logits (at most 65535 rows of 1 to %d)", op, rows, vocab, kChooseMaxVocab);
   const int64_t entries = (history != nullptr ? history_width : 0) + static_cast<int64_t>(bias_token != nullptr ? bias_width : 0);
-  if (entries > kMaxIndex || choose_shared(choose_slice(vocab, kChooseMaxCluster), entries) > kChooseShared)
+  if (entries >= (1 << 30)) return refuse("%s: a history and bias list of %lld entries (below 2^30)", op, static_cast<long long>(entries));
+  if (choose_shared(choose_slice(vocab, kChooseMaxCluster), entries) > kChooseShared)
     return refuse("%s: a history and bias list of %lld entries with %d logits (at most 20000 beyond 390000 logits)", op,
                   static_cast<long long>(entries), vocab);
   if (dtype < kBf16 || dtype > kFp32) return refuse("%s: dtype %d (0 bf16, 1 fp16 or 2 fp32)", op, dtype);

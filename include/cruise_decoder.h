@@ -63,7 +63,8 @@ int32_t cruise_decoder_rotate_store(
  * shared by calls that may overlap (its contents do not matter between calls);
  * NULL where that returns 0.  Other pointers 16-byte aligned (block_table,
  * seq_len, lse 4-byte), strides of q, out and blocks multiples of 8 elements;
- * out must not overlap the inputs; num_blocks block_stride at most 2^35. */
+ * out must not overlap the inputs; num_blocks block_stride at most 2^35,
+ * table_width block_size below 2^31 - 256. */
 int32_t cruise_decoder_attention(
     const void *q, int64_t q_stride, int32_t rows, int32_t num_heads,
     int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
@@ -104,8 +105,8 @@ int64_t cruise_decoder_attention_workspace(int32_t rows, int32_t num_heads,
  * same stride), else must not overlap them.  append: token[r] >= 0 is written to
  * history[r][history_len[r]] where that is inside history_width (history_len
  * itself is the caller's to advance).  4-byte alignment suffices (logits: their
- * own size).  vocab at most 2^20; beyond
- * 390000 at most 20000 history and bias entries together. */
+ * own size).  vocab at most 2^20; fewer than 2^30 history and bias entries
+ * together, beyond 390000 logits at most 20000. */
 int32_t cruise_decoder_choose(
     const void *logits, int64_t logits_stride, int32_t rows, int32_t vocab,
     int32_t dtype, const int32_t *active, int32_t *history,

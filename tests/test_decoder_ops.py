@@ -55,6 +55,9 @@ def test_rotate_store_refuses(change, reason):
     (dict(rows=-1), "rows"), (dict(num_heads=5), "multiple"), (dict(head_dim=32), "head size"),
     (dict(dtype=2), "dtype"), (dict(num_blocks=0), "blocks"), (dict(table_width=-1), "tables"),
     (dict(table_width=1 << 28, table_stride=1 << 28), "capacity"),
+    (dict(rows=1, num_heads=1, num_kv_heads=1, table_width=(2 ** 31 - 200) // 16, table_stride=1 << 28), "capacity"),
+    (dict(rows=8, num_heads=8, num_kv_heads=8, table_width=(2 ** 31 - 320) // 16, table_stride=1 << 28, q_stride=512,
+          out_stride=512, block_stride=8192), "passes 2^31"),
     (dict(rows=1 << 20, table_width=1 << 20, table_stride=1 << 20), "passes 2^31"),
     (dict(table_stride=1), "stride"), (dict(q_stride=252), "stride"), (dict(out_stride=260), "multiples of 8"),
     (dict(num_blocks=1 << 20, block_stride=1 << 16), "2^35"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(out=None), "NULL"),
@@ -79,6 +82,8 @@ def test_attention_refuses(change, reason):
 @pytest.mark.parametrize("change, reason", [
     (dict(rows=-1), "rows"), (dict(rows=70000), "rows"), (dict(vocab=0), "logits"), (dict(vocab=(1 << 20) + 1), "logits"),
     (dict(vocab=1000000, logits_stride=1000000, history_width=30000, history_stride=30000), "entries"),
+    (dict(history_width=1 << 30, history_stride=1 << 30), "entries"),
+    (dict(bias_token=at(6), bias_value=at(7), bias_len=at(8), bias_width=(1 << 30) - 10, bias_stride=1 << 30), "entries"),
     (dict(dtype=3), "dtype"), (dict(logits_stride=99), "stride"), (dict(history_width=11), "history"),
     (dict(history_len=None), "history"), (dict(history=None), "need a history"),
     (dict(history=None, append=0, presence=at(6)), "need a history"),
