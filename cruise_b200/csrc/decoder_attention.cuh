@@ -139,9 +139,10 @@ __host__ __device__ __forceinline__ int row_tiles(int length) {
 }
 
 template <typename T, int D, int NT, int Warps, AttendForm Form>
-__global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warps == 8 ? 1 : Warps == 4 ? 2 : 8) : attend_ctas(D)) attention_kernel(const AttentionPlan p) {
+__global__ void __launch_bounds__(Warps * 32, Form == AttendForm::kSplit ? attend_ctas(D) : Warps == 8 ? 1 : Warps == 4 ? 2 : 8)
+attention_kernel(const AttentionPlan p) {
   using S = AttendShared<D, Warps>;
-  constexpr bool Whole = Form != AttendForm::kSplit, kCluster = Form == AttendForm::kCluster;
+  constexpr bool kOneUnit = Form != AttendForm::kSplit, kCluster = Form == AttendForm::kCluster;
   constexpr int kAttendStages = S::kStages;
   constexpr int kAttendThreads = Warps * 32, kAttendTile = Warps * kAttendKeys;
   // The ring, then the merge's room (a whole unit's CTA merges in the ring).  Two
@@ -153,9 +154,9 @@ __global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warp
   auto factor = [&](int w, int h) -> float & { return NT == 1 ? merge_f_room[w * 8 + h] : merge_ml[w][h][0]; };
   uint32_t *const words = reinterpret_cast<uint32_t *>(ring + S::kRingBytes);
   auto word = [&](int line, int i) -> uint32_t & {   // word i < 4 (8) of 8 * Warps lines
-    return Whole ? words[line * 8 + i] : words[line * S::kMergeStride + D + i];
+    return kOneUnit ? words[line * 8 + i] : words[line * S::kMergeStride + D + i];
   };
-  static_assert(kAttendStages <= (Whole ? 8 : 4), "a line holds a warp's masks");
+  static_assert(kAttendStages <= (kOneUnit ? 8 : 4), "a line holds a warp's masks");
   constexpr int kChunks = D / 8;   // 16-byte chunks of a row
   const AttentionArgs &a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -166,8 +167,8 @@ __global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warp
   // set-up, then its tiles) --
   constexpr int kSetup = attend_setup(D);
   int row, off = 0, left = 1, length0;
-    const int ranks = kCluster ? p.ranks : 1, rank = kCluster ? static_cast<int>(blockIdx.x) : 0;
-  if constexpr (Whole) {
+  const int ranks = kCluster ? p.ranks : 1, rank = kCluster ? static_cast<int>(blockIdx.x) : 0;
+  if constexpr (kOneUnit) {
     // grid: (CTAs of the cluster, units, rows), or (units, rows in y and z)
     row = kCluster ? blockIdx.z : blockIdx.z * gridDim.y + blockIdx.y;
     if (row >= a.rows) return;
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warp
   };
   auto begin_at = [&]() {
     Cursor c{row, off, left, length0, 0};
-    if (!Whole && row + 1 < a.rows) c.length_ahead = row_length(p, row + 1);
+    if (!kOneUnit && row + 1 < a.rows) c.length_ahead = row_length(p, row + 1);
     return c;
   };
   auto next_segment = [&](Cursor &c, Segment &s) {
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warp
       s.row = c.row;
       s.length = c.length;
       s.n = row_tiles<Warps>(s.length);
-      if constexpr (Whole) {
+      if constexpr (kOneUnit) {
         s.unit = kCluster ? blockIdx.y : blockIdx.x;
         s.t0 = rank;   // and every `ranks`-th tile from there, so that the first is known before the length
         s.count = s.n > rank ? (s.n - rank + ranks - 1) / ranks : 0;
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warp
         vsrc = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.value_cache) + kvh * D) + lane % kChunks;
         load_tile = 0;
         next_block = block_of(0);
-        if constexpr (Whole) loading = from.count > 0;
+        if constexpr (kOneUnit) loading = from.count > 0;
       }
     }
     uint32_t mask = 0;
@@ -430,8 +431,8 @@ __global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warp
       fill = fill + 1 == kAttendStages ? 0 : fill + 1;
     }
     // -- the warps' parts of the segment meet in shared memory --
-    if constexpr (Whole) cp_async_wait_all();   // the ring, done with, is the room for it
-    float *const merge = reinterpret_cast<float *>(Whole ? ring : ring + S::kRingBytes);
+    if constexpr (kOneUnit) cp_async_wait_all();   // the ring, done with, is the room for it
+    float *const merge = reinterpret_cast<float *>(kOneUnit ? ring : ring + S::kRingBytes);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -445,11 +446,11 @@ __global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warp
       }
     }
     __syncthreads();   // every warp is done with its products, and with the merge before this one
-    const bool whole = Whole ? !kCluster : t0 == 0 && count == n;
+    const bool whole = kOneUnit ? !kCluster : t0 == 0 && count == n;
     // the cluster's inbox: [rank][head] (m, l), then [rank][join_each] four dimensions of O
     float2 *const inbox_ml = reinterpret_cast<float2 *>(words + Warps * 8);
     float4 *const inbox_o = reinterpret_cast<float4 *>(inbox_ml + kAttendRanks * NT * 8);
-    const int join_each = Whole ? (heads * (D / 4) + ranks - 1) / ranks : 0;
+    const int join_each = kOneUnit ? (heads * (D / 4) + ranks - 1) / ranks : 0;
     if constexpr (kCluster) cluster_wait();
     const int64_t piece = 2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0);
     if (tid < (heads * Warps + 31) / 32 * 32) {   // whole warps: a lane per (head, warp)
@@ -540,8 +541,8 @@ __global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warp
           a.lse[static_cast<int64_t>(row_now) * a.nq + head0 + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
       }
     }
-    if (NT > 1 && !Whole) __syncthreads();   // the factors have been read
-    if (!Whole && t0 == 0) {
+    if (NT > 1 && !kOneUnit) __syncthreads();   // the factors have been read
+    if (!kOneUnit && t0 == 0) {
       const int4 of = make_int4(row_now, unit, whole ? 0 : 1 + (n - count + share_work - 1) / share_work, blockIdx.x);
       if (p.by_unit) {
         if (tid == 0) p.piece_of[row_now * p.units + unit] = of;
@@ -550,7 +551,7 @@ __global__ void __launch_bounds__(Warps * 32, Form != AttendForm::kSplit ? (Warp
       }
     }
   }
-  if (!Whole && !p.by_unit && tid == 0) p.piece_of[blockIdx.x] = tail;
+  if (!kOneUnit && !p.by_unit && tid == 0) p.piece_of[blockIdx.x] = tail;
 }
 
 // Joins the pieces of a split unit (piece_of), `heads_each` of its heads a CTA.

@@ -597,13 +597,14 @@ def test_calls_follow_the_current_stream():
     assert torch.equal(got, want)
 
 
-def test_overlapping_calls_do_not_meet():
+@pytest.mark.parametrize("width", [None, 2000])
+def test_overlapping_calls_do_not_meet(width):
     """Two streams and two threads at once: each call has its own workspace."""
     import threading
 
     from cruise_b200.decoder_ops import paged_attention
 
-    cases = [attend_case([9000 - 37 * i], 8, 2, 64, BF16, width=2000, seed=22 + i) for i in range(4)]
+    cases = [attend_case([9000 - 37 * i], 8, 2, 64, BF16, width=width, seed=22 + i) for i in range(4)]
     wants = [paged_attention(*c.values()) for c in cases]
     torch.cuda.synchronize()
     bad = []
@@ -657,6 +658,49 @@ def test_captured_attention_follows_its_inputs():
         torch.cuda.synchronize()
         for out, want in zip(outs, wants):
             assert torch.equal(out, want)
+
+
+FIRST_CALLS = """
+import torch
+from cruise_b200.decoder_ops import choose, paged_attention
+
+def captured_first(call, out):
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    graph.replay()
+    torch.cuda.synchronize()
+    got = out.clone()
+    call()
+    torch.cuda.synchronize()
+    assert torch.equal(got, out)
+
+cuda = dict(device="cuda")
+key, value = (torch.randn(32, 16, 2, 64, **cuda).bfloat16() for _ in range(2))
+for rows, width in ((2, 100), (2, 3000), (200, 20), (2, 1)):
+    q = torch.randn(rows, 8, 64, **cuda).bfloat16()
+    table = torch.randint(0, 32, (rows, width), dtype=torch.int32, **cuda)
+    lens = torch.full((rows,), width * 16 - 5, dtype=torch.int32, **cuda)
+    out = torch.empty_like(q)
+    captured_first(lambda: paged_attention(q, key, value, table, lens, out=out), out)
+logits, token = torch.randn(3, 50000, **cuda), torch.empty(3, dtype=torch.int64, **cuda)
+captured_first(lambda: choose(logits, out=token), token)
+assert torch.equal(token, logits.argmax(dim=1))
+print("the same")
+"""
+
+
+def test_first_calls_may_be_captured():
+    """In a fresh process: the first call of each form of attention and of choose
+    inside a capture, where the library asks the device for its limits."""
+    import pathlib
+    import subprocess
+    import sys
+
+    root = pathlib.Path(__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "the same" in done.stdout, done.stderr[-2000:]
 
 
 def test_captured_calls_behind_copies_memsets_and_joins():
