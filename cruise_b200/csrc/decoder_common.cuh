@@ -47,6 +47,8 @@ struct Element;
 
 template <>
 struct Element<__nv_bfloat16> {
+  static constexpr float kHalfStep = 0x1p-8f;   // half a step relative to the value: a rounding is off by at most this
+  static constexpr float kLift = 1.f;           // brings values of at most 1 to the top of the range (fp32's here)
   static __device__ __forceinline__ float2 unpack(uint32_t v) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
   }
@@ -66,6 +68,8 @@ struct Element<__nv_bfloat16> {
 
 template <>
 struct Element<__half> {
+  static constexpr float kHalfStep = 0x1p-11f;
+  static constexpr float kLift = 0x1p15f;
   static __device__ __forceinline__ float2 unpack(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&v));
   }
