@@ -1248,13 +1248,18 @@ int32_t run_decoder_step_paged(Engine *e, const PagedStep &s) {
   if ((s.rope_cos == nullptr) != (s.rope_sin == nullptr)) return reject("pass both rotation tables or neither");
   if (s.rope_cos != nullptr && ((s.rope_dtype != ops::kBf16 && s.rope_dtype != ops::kFp32) || s.rope_rows < 1))
     return reject("rotation tables are bf16 (0) or fp32 (2) with at least one row");
-  for (const void *p : {static_cast<const void *>(s.key_cache), static_cast<const void *>(s.value_cache), s.rope_cos, s.rope_sin})
-    if ((reinterpret_cast<uintptr_t>(p) & 15) != 0) return reject("caches and tables must be 16-byte aligned");
-  for (const void *p : {static_cast<const void *>(s.token), static_cast<const void *>(s.position),
-                        static_cast<const void *>(s.key_cache), static_cast<const void *>(s.value_cache),
-                        static_cast<const void *>(s.block_table), static_cast<const void *>(s.logits)}) {
+  const struct {
+    const void *at;
+    uintptr_t bytes;
+  } arrays[] = {{s.key_cache, 16}, {s.value_cache, 16}, {s.rope_cos, 16}, {s.rope_sin, 16},
+                {s.token, 8},      {s.position, 8},     {s.block_table, 4}, {s.logits, 2}};
+  for (const auto &array : arrays)
+    if ((reinterpret_cast<uintptr_t>(array.at) & (array.bytes - 1)) != 0)
+      return reject("caches and tables must be 16-byte aligned, the other arrays to their elements");
+  for (const auto &array : arrays) {
+    if (array.at == nullptr) continue;   // no rotation tables: the engine's
     cudaPointerAttributes attr{};
-    if (cudaPointerGetAttributes(&attr, p) != cudaSuccess || attr.type != cudaMemoryTypeDevice || attr.device != e->device) {
+    if (cudaPointerGetAttributes(&attr, array.at) != cudaSuccess || attr.type != cudaMemoryTypeDevice || attr.device != e->device) {
       cudaGetLastError();
       return reject("every tensor must be device memory on the engine's device");
     }

@@ -292,7 +292,7 @@ int32_t cruise_decoder_step(void *engine, const int64_t *token,
  * [kv_heads][head_dim] (16-byte aligned, updated in place at each position's
  * slot), block_table i32 [rows][table_width] (rows table_stride entries apart),
  * rope_cos / rope_sin [rope_rows][head_dim] of rope_dtype 0 (bf16) or 2 (fp32),
- * or both NULL for the engine's own tables.  A row whose token or position does
+ * (16-byte aligned), or both NULL for the engine's own tables.  A row whose token or position does
  * not exist is inactive too; the logits of inactive rows must not be used.  Two
  * rows must not share a slot.  rows at most 4 block_size of the engine.
  * logits: bf16 [rows][vocab], rows logits_stride elements apart (the decoder's

@@ -1,0 +1,71 @@
+"""The paged decoder step (cruise_decoder_step_paged) at its edges: refusals of
+the C entry before anything is launched."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_decoder_step_paged import GEOMETRY, _pair
+
+pytestmark = pytest.mark.gpu
+
+BLOCK, WIDTH = 16, 4
+
+
+@pytest.fixture(scope="module")
+def engine():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    engine, _, _ = _pair(GEOMETRY, BLOCK, WIDTH)
+    yield engine
+    torch.cuda.synchronize()
+    engine.close()
+
+
+def tensors(rows=4, blocks=16):
+    shape = (GEOMETRY["num_layers"], blocks, BLOCK, GEOMETRY["num_kv_heads"], GEOMETRY["head_dim"])
+    cuda = dict(device="cuda")
+    return dict(token=torch.arange(rows, **cuda), position=torch.arange(rows, **cuda),
+                key=torch.zeros(shape, dtype=torch.bfloat16, **cuda), value=torch.zeros(shape, dtype=torch.bfloat16, **cuda),
+                table=torch.arange(rows * WIDTH, dtype=torch.int32, **cuda).view(rows, WIDTH),
+                cos=torch.ones(BLOCK * WIDTH, 128, **cuda), sin=torch.zeros(BLOCK * WIDTH, 128, **cuda),
+                logits=torch.zeros(rows, GEOMETRY["vocab"], dtype=torch.bfloat16, **cuda))
+
+
+def step(engine, t, **change):
+    """The C call on the tensors' addresses, or on those in ``change``."""
+    at = {name: x.data_ptr() for name, x in t.items()}
+    at.update(change)
+    rows, blocks = t["token"].shape[0], t["key"].shape[1]
+    rc = engine.lib.cruise_decoder_step_paged(
+        engine.handle, rows, at["token"], at["position"], at["key"], at["value"], blocks, BLOCK, at["table"], WIDTH, WIDTH,
+        at["cos"], at["sin"], 2, BLOCK * WIDTH, at["logits"], GEOMETRY["vocab"], torch.cuda.current_stream().cuda_stream)
+    why = engine.lib.cruise_epoch_last_error(engine.handle)
+    return rc, why.decode() if why else ""
+
+
+@pytest.mark.parametrize("name", ["cos", "sin", "token", "position", "key", "value", "table", "logits"])
+def test_host_memory_is_refused(engine, name):
+    t = tensors()
+    host = t[name].cpu()
+    for there in (host, host.pin_memory()):
+        rc, why = step(engine, t, **{name: there.data_ptr()})
+        assert rc == -1 and ("device memory" in why or "aligned" in why), (rc, why)
+    assert not t["key"].any() and not t["logits"].any()
+
+
+@pytest.mark.parametrize("name, off", [("cos", 8), ("sin", 4), ("key", 8), ("value", 2), ("token", 4), ("position", 4),
+                                       ("table", 2), ("logits", 1)])
+def test_unaligned_arrays_are_refused(engine, name, off):
+    t = tensors()
+    rc, why = step(engine, t, **{name: t[name].data_ptr() + off})
+    assert rc == -1 and "aligned" in why, (rc, why)
+    assert not t["key"].any() and not t["logits"].any()
+
+
+def test_the_same_arrays_are_taken(engine):
+    t = tensors()
+    rc, why = step(engine, t)
+    assert rc == 0, why
+    assert t["logits"].any() and t["key"].any()
