@@ -395,16 +395,6 @@ int32_t report(cudaError_t err, const char *what) {
 
 bool aligned(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// Whether [a, a + na) and [b, b + nb) bytes overlap.
-bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return na > 0 && nb > 0 && x < y + static_cast<uintptr_t>(nb) && y < x + static_cast<uintptr_t>(na);
-}
-
-int64_t extent(int64_t rows, int64_t stride, int64_t width, int64_t size) {
-  return rows > 0 ? ((rows - 1) * stride + width) * size : 0;
-}
-
 }  // namespace
 
 cudaError_t launch_rotate_store(const RotateArgs &a, int device, cudaStream_t stream) {

@@ -77,6 +77,17 @@ struct ChooseArgs {
   int32_t append;             // 1: history[r][history_len[r]] = token where it fits
 };
 
+// Whether [a, a + na) and [b, b + nb) bytes overlap.
+inline bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na > 0 && nb > 0 && x < y + static_cast<uintptr_t>(nb) && y < x + static_cast<uintptr_t>(na);
+}
+
+// Bytes from the first to the last element of rows `stride` elements apart.
+inline int64_t extent(int64_t rows, int64_t stride, int64_t width, int64_t size) {
+  return rows > 0 ? ((rows - 1) * stride + width) * size : 0;
+}
+
 cudaError_t launch_rotate_store(const RotateArgs &a, int device, cudaStream_t stream);
 int64_t attention_workspace(int32_t rows, int32_t nq, int32_t nkv, int32_t d, int64_t capacity, int device);
 cudaError_t launch_paged_attention(const AttentionArgs &a, int device, cudaStream_t stream);

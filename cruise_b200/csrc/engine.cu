@@ -1264,6 +1264,20 @@ int32_t run_decoder_step_paged(Engine *e, const PagedStep &s) {
       return reject("every tensor must be device memory on the engine's device");
     }
   }
+  // what the step writes, each apart from the other arrays
+  const int64_t cache_bytes = 2 * m.L * s.num_blocks * s.block_size * static_cast<int64_t>(m.nkv) * m.d;
+  const int64_t rope_bytes = s.rope_cos == nullptr ? 0 : static_cast<int64_t>(s.rope_rows) * m.d * (s.rope_dtype == ops::kBf16 ? 2 : 4);
+  const struct {
+    const void *at;
+    int64_t bytes;
+  } spans[] = {{s.key_cache, cache_bytes}, {s.value_cache, cache_bytes}, {s.logits, ops::extent(s.rows, s.logits_stride, m.V, 2)},
+               {s.token, 8ll * s.rows},    {s.position, 8ll * s.rows},
+               {s.block_table, ops::extent(s.rows, s.table_stride, s.table_width, 4)},
+               {s.rope_cos, rope_bytes},   {s.rope_sin, rope_bytes}};
+  for (int i = 0; i < 3; ++i)
+    for (int j = i + 1; j < 8; ++j)
+      if (ops::overlap(spans[i].at, spans[i].bytes, spans[j].at, spans[j].bytes))
+        return reject("the caches and the logits must not overlap one another or the inputs");
   cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(s.stream, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone) {
     cudaGetLastError();

@@ -294,7 +294,8 @@ int32_t cruise_decoder_step(void *engine, const int64_t *token,
  * rope_cos / rope_sin [rope_rows][head_dim] of rope_dtype 0 (bf16) or 2 (fp32),
  * (16-byte aligned), or both NULL for the engine's own tables.  A row whose token or position does
  * not exist is inactive too; the logits of inactive rows must not be used.  Two
- * rows must not share a slot.  rows at most 4 block_size of the engine.
+ * rows must not share a slot, and the caches and the logits must not overlap one
+ * another or the inputs.  rows at most 4 block_size of the engine.
  * logits: bf16 [rows][vocab], rows logits_stride elements apart (the decoder's
  * rounding: cruise_decoder_step gives the same values as f32).  Rounds where the
  * decoder does, but for the attention's scores and probabilities and the

@@ -64,6 +64,29 @@ def test_unaligned_arrays_are_refused(engine, name, off):
     assert not t["key"].any() and not t["logits"].any()
 
 
+@pytest.mark.parametrize("name, other, off", [
+    ("value", "key", 0), ("value", "key", 4096), ("key", "value", 64), ("logits", "key", 0), ("logits", "value", 65536),
+    ("token", "key", 128), ("position", "value", 8), ("table", "key", 4), ("cos", "key", 256), ("sin", "value", 0),
+    ("logits", "token", 0), ("logits", "position", 16), ("logits", "table", 4), ("cos", "logits", 512), ("sin", "logits", 0),
+])
+def test_overlapping_arrays_are_refused(engine, name, other, off):
+    t = tensors()
+    rc, why = step(engine, t, **{name: t[other].data_ptr() + off})
+    assert rc == -1 and "overlap" in why, (rc, why)
+    assert not t["key"].any() and not t["logits"].any()
+
+
+def test_arrays_side_by_side_are_taken(engine):
+    t = tensors()
+    want = {name: x.clone() for name, x in t.items()}
+    assert step(engine, want)[0] == 0
+    both = torch.zeros(2, *t["key"].shape, dtype=torch.bfloat16, device="cuda")
+    t.update(key=both[0], value=both[1])
+    rc, why = step(engine, t)
+    assert rc == 0, why
+    assert torch.equal(t["logits"], want["logits"]) and torch.equal(t["key"], want["key"]) and torch.equal(t["value"], want["value"])
+
+
 def test_the_same_arrays_are_taken(engine):
     t = tensors()
     rc, why = step(engine, t)
