@@ -171,7 +171,9 @@ struct PrefillState {
   float *acc = nullptr;        // fp32 k-range partial sums [split][T][N]
   int64_t *tok = nullptr;
   int32_t *row = nullptr, *pos = nullptr;
-  uint32_t *error = nullptr;   // site of a tensor-core GEMM wait that ran out (0: none)
+  // site of a tensor-core GEMM wait that ran out (0: none); then the first row that a
+  // paged decoder step left out (prefill::paged_rows)
+  uint32_t *error = nullptr;
   bool chain = true;           // kernels launched as programmatic dependents (CRUISE_PREFILL_PDL=0: plain)
   int narrow_tile = 0;         // token tile cap of QKV, O and down (CRUISE_PREFILL_TTILE; 0: all tokens)
   int force_split = 0;         // their split count (CRUISE_PREFILL_SPLIT; 0: the cost model's)
@@ -1017,7 +1019,7 @@ int32_t prefill_prepare(Engine *e) {
   const size_t o_h = take(T * H * 2), o_x = take(T * H * 2), o_q = take(T * Hq * 2), o_attn = take(T * Hq * 2);
   const size_t o_act = take(T * I * 2), o_y = take(T * H * 2), o_acc = take(parts * 4), o_tok = take(T * 8),
                o_row = take(T * 4),
-               o_pos = take(T * 4), o_err = take(4);
+               o_pos = take(T * 4), o_err = take(8);
   cudaError_t err = cudaMalloc(&ps->work, bytes);
   if (err != cudaSuccess) return set_err(e, err, "prefill buffers");
   uint8_t *b = static_cast<uint8_t *>(ps->work);
@@ -1309,6 +1311,7 @@ int32_t run_decoder_step_paged(Engine *e, const PagedStep &s) {
   cudaError_t err = cudaEventRecord(pg->before, s.stream);
   if (err == cudaSuccess) err = cudaStreamWaitEvent(e->stream, pg->before, 0);
   if (err == cudaSuccess) err = cudaMemsetAsync(ps->error, 0, 4, e->stream);
+  if (err == cudaSuccess) err = cudaMemsetAsync(ps->error + 1, 0xff, 4, e->stream);
   if (err != cudaSuccess) return set_err(e, err, "paged decoder step inputs");
   const GemmPlan pq = gemm_plan(e, N, H, T), po = gemm_plan(e, H, m.Hq, T);
   const GemmPlan pg_up = gemm_plan(e, 2 * I, H, T, false), pd = gemm_plan(e, H, m.I_pad, T);
@@ -1355,7 +1358,8 @@ int32_t run_decoder_step_paged(Engine *e, const PagedStep &s) {
   aa.workspace = pg->attention;
   const int64_t layer_elems = s.num_blocks * ra.block_stride;
   prefill::paged_rows<<<T, 128, 0, e->stream>>>(e->embed, s.token, s.position, s.block_table, s.table_stride, s.table_width,
-                                                s.block_size, s.num_blocks, rope_rows, m.V, ps->h, pg->slot, pg->length, H);
+                                                s.block_size, s.num_blocks, rope_rows, m.V, ps->h, pg->slot, pg->length,
+                                                ps->error + 1, H);
   chain_launch(e, T, 256, 0, prefill::rms_norm_rows, ps->h, e->layers[0].w_in, ps->x, H, m.eps);
   bool gemm_ok = true;
   for (int l = 0; l < m.L && gemm_ok && err == cudaSuccess; ++l) {
@@ -1391,16 +1395,22 @@ int32_t run_decoder_step_paged(Engine *e, const PagedStep &s) {
   if (err == cudaSuccess)
     err = cudaMemcpy2DAsync(s.logits, s.logits_stride * 2, pg->logits, static_cast<size_t>(m.V_pad) * 2, static_cast<size_t>(m.V) * 2,
                             T, cudaMemcpyDeviceToDevice, e->stream);
-  uint32_t site = 0;
-  if (err == cudaSuccess) err = cudaMemcpyAsync(&site, ps->error, 4, cudaMemcpyDeviceToHost, e->stream);
+  uint32_t status[2] = {0, UINT32_MAX};   // a GEMM wait's site, the first row left out
+  if (err == cudaSuccess) err = cudaMemcpyAsync(status, ps->error, 8, cudaMemcpyDeviceToHost, e->stream);
   if (err == cudaSuccess) err = cudaEventRecord(pg->after, e->stream);
   if (err == cudaSuccess) err = cudaStreamWaitEvent(s.stream, pg->after, 0);
   const cudaError_t done = cudaStreamSynchronize(e->stream);   // (also after a failure: the buffers are free again)
   if (err == cudaSuccess) err = done;
   if (err != cudaSuccess) return set_err(e, err, "paged decoder step");
-  if (site != 0) {
-    e->last_error = "cruise_decoder_step_paged: a tensor-core GEMM wait gave up (site " + std::to_string(site) + ")";
+  if (status[0] != 0) {
+    e->last_error = "cruise_decoder_step_paged: a tensor-core GEMM wait gave up (site " + std::to_string(status[0]) + ")";
     return -3;
+  }
+  if (status[1] != UINT32_MAX) {
+    e->last_error = "cruise_decoder_step_paged: left out row " + std::to_string(status[1] / 2) +
+                    (status[1] % 2 != 0 ? ", whose position lies past the rotation tables (" + std::to_string(rope_rows) + " rows)"
+                                        : ", whose position's table entry is no block of the cache");
+    return -5;
   }
   return 0;
 }

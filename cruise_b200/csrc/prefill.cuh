@@ -330,18 +330,23 @@ __global__ void qkv_rope_store(const float *acc, int nsplit, int T, const bf16 *
 // First kernel of a decoder step over caller-held paged caches, one CTA per
 // row: h = embed[token]; slot and length of the row's position.  A row whose
 // position is negative or past its table, or whose token does not exist, is
-// inactive: h is zero, nothing is stored (slot -1) and it attends to nothing.
+// inactive: h is zero, nothing is stored (slot -1) and it attends to nothing.  So
+// is one whose position has no block in the cache or no row in the rotation
+// tables, but that is the caller's mistake: the first such row goes to `left_out`
+// (all bits set: none) as 2 row, plus 1 for the tables.
 __global__ void paged_rows(const bf16 *embed, const int64_t *token, const int64_t *position, const int32_t *table,
                            int64_t table_stride, int32_t table_width, int32_t block_size, int64_t num_blocks,
-                           int32_t rope_rows, int32_t vocab, bf16 *h, int32_t *slot, int32_t *length, int H) {
+                           int32_t rope_rows, int32_t vocab, bf16 *h, int32_t *slot, int32_t *length, uint32_t *left_out,
+                           int H) {
   const int t = blockIdx.x;
   const int64_t id = token[t], pos = position[t];
-  const bool active = id >= 0 && id < vocab && pos >= 0 && pos < rope_rows &&
-                      pos < static_cast<int64_t>(table_width) * block_size;
+  const bool asked = id >= 0 && id < vocab && pos >= 0 && pos < static_cast<int64_t>(table_width) * block_size;
+  const int64_t block = asked ? table[t * table_stride + pos / block_size] : -1;
+  const bool turns = pos < rope_rows, active = asked && turns && block >= 0 && block < num_blocks;
   if (threadIdx.x == 0) {
-    const int64_t block = active ? table[t * table_stride + pos / block_size] : -1;
-    slot[t] = block >= 0 && block < num_blocks ? static_cast<int32_t>(block * block_size + pos % block_size) : -1;
+    slot[t] = active ? static_cast<int32_t>(block * block_size + pos % block_size) : -1;
     length[t] = active ? static_cast<int32_t>(pos + 1) : 0;
+    if (asked && !active) atomicMin(left_out, 2u * t + (turns ? 0 : 1));
   }
   const uint4 *src = reinterpret_cast<const uint4 *>(embed + (active ? id : 0) * static_cast<int64_t>(H));
   uint4 *dst = reinterpret_cast<uint4 *>(h + static_cast<int64_t>(t) * H);

@@ -270,7 +270,7 @@ class EpochEngine:
     def decoder_step_paged(self, token: torch.Tensor, position: torch.Tensor, block_table: torch.Tensor,
                            key: torch.Tensor, value: torch.Tensor, cos: torch.Tensor | None = None,
                            sin: torch.Tensor | None = None, logits_out: torch.Tensor | None = None) -> torch.Tensor:
-        """One decoder step of any number of rows over caller-held paged caches of
+        """One decoder step of many rows over caller-held paged caches of
         any length (``cruise_decoder_step_paged``): the engine's projections
         around :func:`cruise_b200.decoder_ops.rotate_store` and
         :func:`cruise_b200.decoder_ops.paged_attention`.  CUDA tensors on the
@@ -278,8 +278,12 @@ class EpochEngine:
         position: the row is inactive), ``block_table`` int32 [rows, width],
         ``key`` / ``value`` bf16 [layers, blocks, block_size, kv heads, head_dim]
         (updated in place), ``cos`` / ``sin`` [positions, head_dim] bf16 or fp32
-        (the engine's tables by default).  Returns the logits bf16 [rows, V]
-        (``logits_out``); :func:`cruise_b200.decoder_ops.choose` takes them."""
+        (the engine's tables by default, which end at its own ``capacity``; at
+        most 4 * block_size rows of its configuration).  Returns the logits bf16
+        [rows, V] (``logits_out``); :func:`cruise_b200.decoder_ops.choose` takes
+        them.  A position past the rotation tables, or whose table entry is no
+        block of the caches, raises once the step has completed for the other
+        rows."""
         cfg = self.config
         tensors = dict(token=token, position=position, block_table=block_table, key=key, value=value, cos=cos, sin=sin,
                        logits_out=logits_out)

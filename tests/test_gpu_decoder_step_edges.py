@@ -87,6 +87,65 @@ def test_arrays_side_by_side_are_taken(engine):
     assert torch.equal(t["logits"], want["logits"]) and torch.equal(t["key"], want["key"]) and torch.equal(t["value"], want["value"])
 
 
+def rows_left_out(engine, **change):
+    """The step with a row 2 that has to be left out against the step without it."""
+    t = tensors()
+    want = {name: x.clone() for name, x in t.items()}
+    want["position"][2] = -1
+    assert step(engine, want)[0] == 0
+    for name, value in change.items():
+        t[name] = value(t[name])
+    rc, why = step(engine, t)
+    assert torch.equal(t["key"], want["key"]) and torch.equal(t["value"], want["value"])
+    others = [0, 1, 3]
+    assert torch.equal(t["logits"][others], want["logits"][others])
+    return rc, why
+
+
+@pytest.mark.parametrize("entry", [-1, 16, 2 ** 31 - 1, -2 ** 31])
+def test_a_position_without_a_block_is_an_error(engine, entry):
+    def spoil(table):
+        table[2, 0] = entry
+        return table
+
+    rc, why = rows_left_out(engine, table=spoil)
+    assert rc == -5 and "row 2" in why and "block" in why, (rc, why)
+
+
+def test_a_position_past_the_rotation_tables_is_an_error(engine):
+    from cruise_b200.engine import EngineError
+
+    t = tensors()
+    t["position"][2] = 40
+    t["cos"], t["sin"] = t["cos"][:40], t["sin"][:40]
+    want = {name: x.clone() for name, x in t.items()}
+    want["position"][2] = -1
+    call = lambda t, **keep: engine.decoder_step_paged(t["token"], t["position"], t["table"], t["key"], t["value"], **keep)  # noqa: E731
+    logits = call(want, cos=want["cos"], sin=want["sin"])
+    with pytest.raises(EngineError, match=r"\(-5\).*row 2.*rotation tables \(40 rows\)"):
+        call(t, cos=t["cos"], sin=t["sin"], logits_out=t["logits"])
+    assert torch.equal(t["key"], want["key"]) and torch.equal(t["value"], want["value"])
+    assert torch.equal(t["logits"][[0, 1, 3]], logits[[0, 1, 3]])
+    # the engine's own tables end where its resident rows do
+    t = tensors(rows=2, blocks=24)
+    t["table"] = torch.arange(24, dtype=torch.int32, device="cuda").view(2, 12)
+    t["position"][:] = torch.tensor([127, 128])
+    with pytest.raises(EngineError, match=r"row 1.*\(128 rows\)"):
+        call(t)
+    t["position"][1] = 126
+    call(t)
+
+
+def test_rows_that_do_not_exist_stay_inactive(engine):
+    t = tensors()
+    t["token"][0], t["token"][1] = -1, GEOMETRY["vocab"]
+    t["position"][2], t["position"][3] = -5, BLOCK * WIDTH
+    t["table"][:] = -1
+    rc, why = step(engine, t)
+    assert rc == 0, why
+    assert not t["key"].any() and not t["value"].any()
+
+
 def test_the_same_arrays_are_taken(engine):
     t = tensors()
     rc, why = step(engine, t)
