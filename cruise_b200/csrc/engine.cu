@@ -2214,11 +2214,14 @@ int32_t cruise_decoder_step_paged(void *engine, int32_t rows, const int64_t *tok
                                   int64_t table_stride, int32_t table_width, const void *rope_cos, const void *rope_sin,
                                   int32_t rope_dtype, int32_t rope_rows, uint16_t *logits, int64_t logits_stride,
                                   void *stream) {
-  if (engine == nullptr || token == nullptr || position == nullptr || key_cache == nullptr || value_cache == nullptr ||
-      block_table == nullptr || logits == nullptr)
-    return -1;
+  if (engine == nullptr) return -1;
   Engine *e = static_cast<Engine *>(engine);
   std::lock_guard<std::mutex> lock(e->execute_mutex);
+  if (token == nullptr || position == nullptr || key_cache == nullptr || value_cache == nullptr || block_table == nullptr ||
+      logits == nullptr) {
+    e->last_error = "cruise_decoder_step_paged: a required pointer is NULL";
+    return -1;
+  }
   cudaSetDevice(e->device);
   const cruise::PagedStep step{rows, token, position, static_cast<cruise::bf16 *>(key_cache),
                                static_cast<cruise::bf16 *>(value_cache), num_blocks, block_size, block_table, table_stride,

@@ -55,6 +55,12 @@ def test_host_memory_is_refused(engine, name):
     assert not t["key"].any() and not t["logits"].any()
 
 
+@pytest.mark.parametrize("name", ["token", "position", "key", "value", "table", "logits"])
+def test_missing_arrays_are_refused(engine, name):
+    rc, why = step(engine, tensors(), **{name: None})
+    assert rc == -1 and "NULL" in why, (rc, why)
+
+
 @pytest.mark.parametrize("name, off", [("cos", 8), ("sin", 4), ("key", 8), ("value", 2), ("token", 4), ("position", 4),
                                        ("table", 2), ("logits", 1)])
 def test_unaligned_arrays_are_refused(engine, name, off):
