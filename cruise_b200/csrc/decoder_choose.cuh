@@ -3,7 +3,7 @@
 // Per row, for every token n of the vocabulary, in fp32 and in this order:
 //   x = logit (+ the token's bias);
 //   in the row's history (prompt or output): x = x > 0 ? x / repetition : x * repetition;
-//   x = x - frequency * count, x = x - presence * [count > 0], count its occurrences in the output;
+//   count > 0, its occurrences in the output: x = x - frequency * count, x = x - presence;
 //   not allowed by the row's bit mask: x = -inf.
 // The choice is the first maximum above -inf: -1 where there is none, -2 where
 // an x is NaN or +inf.  Each step is one rounded fp32 operation, so the choice

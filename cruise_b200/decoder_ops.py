@@ -98,8 +98,8 @@ def choose(logits: torch.Tensor, *, history: torch.Tensor | None = None, prompt_
     this order: plus its ``bias_value`` (lists ``bias_token`` int32 / ``bias_value``
     fp32 [rows, width], the first ``bias_len[r]`` entries, tokens
     increasing; entries of one token add up); when in the row's history, divided (x > 0) or multiplied by
-    ``repetition[r]``; minus ``frequency[r]`` times its occurrences in the output,
-    minus ``presence[r]`` when it occurs there; -inf when its bit of ``allowed``
+    ``repetition[r]``; when it occurs in the output, minus ``frequency[r]`` times
+    its occurrences there and minus ``presence[r]``; -inf when its bit of ``allowed``
     (int32 [rows, ceil(vocab / 32)], bit n % 32 of word n // 32) is 0.  The history
     int32 [rows, width] holds ``history_len[r]`` tokens, the first
     ``prompt_len[r]`` of them the prompt; ids outside the vocabulary do not count.

@@ -87,8 +87,9 @@ int64_t cruise_decoder_attention_workspace(int32_t rows, int32_t num_heads,
  * For every token, in fp32 and in this order:
  *   x = logit, plus bias_value where the token is in the row's bias list;
  *   token in the history: x = x > 0 ? x / repetition : x * repetition;
- *   x = x - frequency * count; x = x - presence where count > 0;
+ *   count > 0: x = x - frequency * count; x = x - presence;
  *   allowed bit 0: x = -inf.
+ * (So an infinite or NaN penalty acts on the tokens it is for, and no others.)
  * history [rows][history_width] (rows history_stride entries apart) holds
  * history_len[r] tokens, the first prompt_len[r] of them the prompt; count is
  * the token's occurrences after the prompt.  Entries outside the vocabulary do

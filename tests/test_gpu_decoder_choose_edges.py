@@ -64,3 +64,30 @@ def test_infinite_logits_under_a_negative_repetition_in_place():
     assert torch.equal(choose(**case, processed=case["logits"]), token32)
     same = (case["logits"] == x32) | (case["logits"].isnan() & x32.isnan())
     assert same.all()
+
+
+def test_penalties_that_are_not_finite_act_on_the_tokens_they_are_for():
+    """frequency and presence change tokens that occur in the output, repetition
+    those of the history, and no others: infinite and NaN ones too."""
+    from cruise_b200.decoder_ops import choose
+
+    case = choose_case(7, 3001, FP32, bias=0, mask=True, seed=62)
+    case["history_len"][:] = 20
+    case["prompt_len"][:] = 5
+    for r, (name, value) in enumerate([("frequency", math.inf), ("frequency", -math.inf), ("frequency", math.nan),
+                                       ("presence", math.inf), ("presence", math.nan), ("repetition", math.inf),
+                                       ("repetition", math.nan)]):
+        case[name][r] = value
+    check_choose(case)
+    room = torch.empty(7, 3001, device="cuda")
+    token = choose(**case, processed=room)
+    for r in range(7):
+        output = case["history"][r, 5:20].long()
+        output = output[(output >= 0) & (output < 3001)]
+        untouched = torch.ones(3001, dtype=torch.bool, device="cuda")
+        seen = case["history"][r, :20].long()
+        untouched[seen[(seen >= 0) & (seen < 3001)]] = False
+        allowed = (case["allowed"][r, torch.arange(3001, device="cuda") >> 5] >> (torch.arange(3001, device="cuda") & 31)) & 1 != 0
+        assert torch.equal(room[r][untouched & allowed], case["logits"][r][untouched & allowed])
+        if r in (0, 3):   # an infinite penalty bans what was said
+            assert (room[r][output] == -math.inf).all() and int(token[r]) not in output.tolist() and token[r] >= 0
