@@ -393,6 +393,30 @@ int32_t report(cudaError_t err, const char *what) {
   return static_cast<int32_t>(err);
 }
 
+// An array, from its first byte to its last; whether two meet (one of `a` and one of `b`).
+struct Span {
+  const void *at;
+  int64_t bytes;
+};
+bool meets(const Span &a, const Span &b) { return overlap(a.at, a.bytes, b.at, b.bytes); }
+template <size_t N, size_t M>
+bool meets(const Span (&a)[N], const Span (&b)[M]) {
+  for (const Span &x : a)
+    for (const Span &y : b)
+      if (meets(x, y)) return true;
+  return false;
+}
+
+// Whether a block of `a` overlaps one of `b`: both have n blocks of `bytes`, `stride`
+// bytes apart, and may lie between one another (the two caches in one tensor).
+bool blocks_overlap(const void *a, const void *b, int64_t n, int64_t stride, int64_t bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  const uint64_t apart = x < y ? y - x : x - y, blocks = apart / stride, rest = apart % stride;
+  const uint64_t last = static_cast<uint64_t>(n) - 1;   // block i of the lower one meets block i - blocks (- 1) of the other
+  return (blocks <= last && rest < static_cast<uint64_t>(bytes)) ||
+         (blocks + 1 <= last && static_cast<uint64_t>(stride) - rest < static_cast<uint64_t>(bytes));
+}
+
 bool aligned(const void *p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 }  // namespace
@@ -470,11 +494,16 @@ int32_t cruise_decoder_rotate_store(const void *qkv, int64_t qkv_stride, int32_t
     return refuse("%s: pointers must be 16-byte aligned (position 8, slot 4)", op);
   const int64_t in_bytes = extent(tokens, qkv_stride, width, 2), out_bytes = extent(tokens, q_stride, q_width, 2);
   const int64_t cache_bytes = extent(num_blocks, block_stride, block_elems, 2);
-  if (overlap(q_out, out_bytes, qkv, in_bytes) || overlap(key_cache, cache_bytes, qkv, in_bytes) ||
-      overlap(value_cache, cache_bytes, qkv, in_bytes) || overlap(q_out, out_bytes, key_cache, cache_bytes) ||
-      overlap(q_out, out_bytes, value_cache, cache_bytes))
-    return refuse("%s: q_out, the caches and qkv must not overlap", op);
+  const int64_t rope_bytes = static_cast<int64_t>(rope_rows) * rotary * (rope_dtype == kFp32 ? 4 : 2);
+  const Span written[] = {{q_out, out_bytes}, {key_cache, cache_bytes}, {value_cache, cache_bytes}};
+  const Span read[] = {{qkv, in_bytes},         {position, 8ll * tokens},   {slot, 4ll * tokens},
+                       {rope_cos, rope_bytes},  {rope_sin, rope_bytes},     {q_norm, q_norm != nullptr ? 2 * head_dim : 0},
+                       {k_norm, k_norm != nullptr ? 2 * head_dim : 0}};
+  if (meets(written, read) || meets(written[0], written[1]) || meets(written[0], written[2]))
+    return refuse("%s: q_out and the caches must not overlap the inputs, nor q_out the caches", op);
   if (key_cache == value_cache) return refuse("%s: the two caches must not be one", op);
+  if (blocks_overlap(key_cache, value_cache, num_blocks, 2 * block_stride, 2 * block_elems))
+    return refuse("%s: the blocks of the two caches must not overlap", op);
   DeviceScope scope(device);
   if (scope.error != cudaSuccess) return report(scope.error, op);
   RotateArgs a{qkv, qkv_stride, tokens, num_heads, num_kv_heads, head_dim, dtype, position, slot, q_norm, k_norm, eps,

@@ -39,7 +39,9 @@ extern "C" {
  * position outside [0, rope_rows) stores nothing and gives zeros in q_out.
  * Two tokens must not have the same slot (either's values may stay).
  * Pointers 16-byte aligned, strides multiples of 8 elements; q_out and the
- * caches must not overlap qkv. */
+ * caches must not overlap the inputs, nor q_out the caches (from first to last
+ * byte), nor a block of one cache a block of the other (the blocks may
+ * alternate). */
 int32_t cruise_decoder_rotate_store(
     const void *qkv, int64_t qkv_stride, int32_t tokens, int32_t num_heads,
     int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
