@@ -626,21 +626,29 @@ int32_t cruise_decoder_choose(const void *logits, int64_t logits_stride, int32_t
       !aligned(presence, 4) || !aligned(bias_token, 4) || !aligned(bias_value, 4) || !aligned(bias_len, 4) ||
       !aligned(allowed, 4) || !aligned(processed, 4))
     return refuse("%s: a pointer is not aligned to its element", op);
-  const int64_t logits_bytes = extent(rows, logits_stride, vocab, size);
-  if (processed != nullptr) {
-    const bool in_place = static_cast<const void *>(processed) == logits && dtype == kFp32 && processed_stride == logits_stride;
-    if (!in_place && overlap(processed, extent(rows, processed_stride, vocab, 4), logits, logits_bytes))
-      return refuse("%s: processed must be the fp32 logits themselves or not overlap them", op);
-  }
-  const int64_t processed_bytes = processed != nullptr ? extent(rows, processed_stride, vocab, 4) : 0;
-  const int64_t history_bytes = history != nullptr ? extent(rows, history_stride, history_width, 4) : 0;
-  const int64_t allowed_bytes = allowed != nullptr ? extent(rows, allowed_stride, (vocab + 31) / 32, 4) : 0;
-  const int64_t bias_bytes = bias_token != nullptr ? extent(rows, bias_stride, bias_width, 4) : 0;
-  if (overlap(processed, processed_bytes, history, history_bytes) || overlap(processed, processed_bytes, allowed, allowed_bytes) ||
-      overlap(processed, processed_bytes, bias_token, bias_bytes) || overlap(processed, processed_bytes, bias_value, bias_bytes) ||
-      overlap(token, 8ll * rows, logits, logits_bytes) || overlap(token, 8ll * rows, history, history_bytes) ||
-      overlap(token, 8ll * rows, processed, processed_bytes) || overlap(token, 8ll * rows, allowed, allowed_bytes) ||
-      (append != 0 && (overlap(history, history_bytes, logits, logits_bytes) || overlap(history, history_bytes, allowed, allowed_bytes))))
+  const int64_t per_row = 4ll * rows;   // bytes of a vector of 32-bit values
+  auto span = [](const void *p, int64_t bytes) { return Span{p, p != nullptr ? bytes : 0}; };
+  auto rows_of = [&](const void *p, int64_t stride, int64_t width, int64_t bytes) { return span(p, extent(rows, stride, width, bytes)); };
+  const Span logits_span = rows_of(logits, logits_stride, vocab, size), history_span = rows_of(history, history_stride, history_width, 4);
+  const Span processed_span = rows_of(processed, processed_stride, vocab, 4), token_span = span(token, 8ll * rows);
+  const bool has_bias = bias_token != nullptr;
+  const Span rules[] = {rows_of(allowed, allowed_stride, (vocab + 31) / 32, 4),
+                        rows_of(bias_token, bias_stride, bias_width, 4),
+                        has_bias ? rows_of(bias_value, bias_stride, bias_width, 4) : Span{},
+                        has_bias ? span(bias_len, per_row) : Span{},
+                        history != nullptr ? span(prompt_len, per_row) : Span{},
+                        history != nullptr ? span(history_len, per_row) : Span{},
+                        span(repetition, per_row),
+                        span(frequency, per_row),
+                        span(presence, per_row),
+                        span(active, per_row)};
+  const bool in_place = static_cast<const void *>(processed) == logits && dtype == kFp32 && processed_stride == logits_stride;
+  if (!in_place && meets(processed_span, logits_span))
+    return refuse("%s: processed must be the fp32 logits themselves or not overlap them", op);
+  // rows write while others read: every output apart from every input
+  const Span outputs[] = {token_span, processed_span}, appended[] = {append != 0 ? history_span : Span{}};
+  if (meets(outputs, rules) || meets(appended, rules) || meets(appended[0], logits_span) || meets(token_span, logits_span) ||
+      meets(token_span, history_span) || meets(processed_span, history_span) || meets(token_span, processed_span))
     return refuse("%s: token, processed and the history must not overlap the inputs", op);
   DeviceScope scope(device);
   if (scope.error != cudaSuccess) return report(scope.error, op);

@@ -105,7 +105,8 @@ int64_t cruise_decoder_attention_workspace(int32_t rows, int32_t num_heads,
  * token[r] = the first maximum above -inf; -1 where there is none; -2 where a
  * processed value is NaN or +inf.  processed (may be NULL) [rows][vocab] fp32,
  * rows processed_stride apart: the x; it may be the logits themselves (fp32,
- * same stride), else must not overlap them.  append: token[r] >= 0 is written to
+ * same stride), else must not overlap them.  token, processed and, with append,
+ * history must not overlap one another or the other inputs.  append: token[r] >= 0 is written to
  * history[r][history_len[r]] where that is inside history_width (history_len
  * itself is the caller's to advance).  4-byte alignment suffices (logits: their
  * own size).  vocab at most 2^20; fewer than 2^30 history and bias entries

@@ -7,7 +7,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_decoder_ops import ROTATE, at, call
+from test_decoder_ops import CHOOSE, ROTATE, at, call
 
 NORMS = dict(q_norm=at(8), k_norm=at(9))
 # rotate_store's sizes: qkv 4 rows of 512, q_out 4 of 256, caches 8 blocks of 2048 elements (4096 bytes), tables of 4096 bytes
@@ -45,3 +45,29 @@ def test_rotate_store_takes_caches_that_alternate(change):
         pytest.skip("made-up addresses: the call would launch")
     rc, why = call("cruise_decoder_rotate_store", {**ROTATE, **change})
     assert rc > 0, why   # no device: past every check
+
+
+# choose's sizes: logits 4 rows of 100 fp32, history 4 of 10, vectors of 4, processed 1600 bytes, token 32
+EVERY = dict(processed=at(5), processed_stride=100, active=at(6), repetition=at(7), frequency=at(8), presence=at(9),
+             bias_token=at(10), bias_value=at(11), bias_len=at(12), bias_width=5, bias_stride=6, allowed=at(13), allowed_stride=4)
+
+
+@pytest.mark.parametrize("name", ["active", "repetition", "frequency", "presence", "bias_token", "bias_value", "bias_len",
+                                  "allowed", "prompt_len", "history_len"])
+@pytest.mark.parametrize("output, last", [("token", 28), ("processed", 1596), ("history", 156)])
+def test_choose_refuses_outputs_over_inputs(name, output, last):
+    base = {**CHOOSE, **EVERY}
+    for off in (0, last):
+        rc, why = call("cruise_decoder_choose", {**base, name: base[output] + off})
+        assert rc == -1 and "overlap" in why, (rc, why)
+    rc, why = call("cruise_decoder_choose", {**base, output: base[name] + 8})
+    assert rc == -1 and "overlap" in why, (rc, why)
+
+
+def test_choose_takes_neighbours_and_a_history_it_only_reads():
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses: the call would launch")
+    for change in (dict(active=at(4) + 32), dict(repetition=at(5) + 1600), dict(presence=at(1) + 160),
+                   dict(append=0, history_len=at(1) + 8), dict(repetition=at(9), presence=at(9)), dict(processed=at(0))):
+        rc, why = call("cruise_decoder_choose", {**CHOOSE, **EVERY, **change})
+        assert rc > 0, why   # no device: past every check
