@@ -96,6 +96,8 @@ class Call {
     NEED(t.layout() == at::kStrided && !t.is_conj() && !t.is_neg(), "%s must be a plain strided tensor", name);
     NEED(!(t.requires_grad() && c10::GradMode::is_enabled()),
          "%s requires a gradient: the decoder operators are for inference", name);
+    // (a view of a traced or fake tensor has an address, an offset from nowhere)
+    NEED(t.numel() == 0 || (t.has_storage() && t.storage().data() != nullptr), "%s has no memory: the call cannot be traced", name);
   }
   int device_ = -1;
 };
