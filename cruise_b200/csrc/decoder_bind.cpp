@@ -13,6 +13,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -96,6 +97,8 @@ class Call {
     NEED(t.layout() == at::kStrided && !t.is_conj() && !t.is_neg(), "%s must be a plain strided tensor", name);
     NEED(!(t.requires_grad() && c10::GradMode::is_enabled()),
          "%s requires a gradient: the decoder operators are for inference", name);
+    NEED(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()),
+         "%s carries a tangent (forward mode): the decoder operators are for inference", name);
     // (a view of a traced or fake tensor has an address, an offset from nowhere)
     NEED(t.numel() == 0 || (t.has_storage() && t.storage().data() != nullptr), "%s has no memory: the call cannot be traced", name);
   }

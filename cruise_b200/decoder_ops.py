@@ -9,7 +9,8 @@ step for the engine's four rows.
 Calls run on the current stream of their tensors' device, queue their kernels
 and return without waiting; they may be captured into a CUDA graph.  They keep
 no state between calls.  They are inference operators: a tensor that requires
-a gradient is refused while gradients are recorded.  Arguments that do not fit
+a gradient is refused while gradients are recorded, and one that carries a
+forward-mode tangent; ``torch.compile`` runs them between its graphs.  Arguments that do not fit
 raise ``ValueError``, failures of the library :class:`DecoderOpError`.  There is
 no fallback without the built library.
 """

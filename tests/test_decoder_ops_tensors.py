@@ -34,3 +34,17 @@ def test_tensors_without_memory_are_refused(call):
     for view in (lambda t: t[:2], lambda t: t[1:]):   # the second has an address, an offset from NULL
         with FakeTensorMode(), pytest.raises(ValueError, match="has no memory"):
             call(view)
+
+
+@pytest.mark.parametrize("call", [attend, rotate, choose])
+def test_forward_mode_tangents_are_refused(call):
+    import torch.autograd.forward_ad as forward
+
+    dual = lambda t: forward.make_dual(t[:2], torch.empty_like(t[:2]))  # noqa: E731
+    with FakeTensorMode():
+        with forward.dual_level(), pytest.raises(ValueError, match="tangent"):
+            call(dual)
+        with forward.dual_level(), torch.no_grad(), pytest.raises(ValueError, match="tangent"):   # it does not stop forward mode
+            call(dual)
+        with forward.dual_level(), pytest.raises(ValueError, match="has no memory"):   # the primal alone is fine
+            call(lambda t: forward.unpack_dual(dual(t)).primal)
