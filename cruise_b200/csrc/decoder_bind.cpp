@@ -208,6 +208,12 @@ int32_t unlocked(F call) {
   return rc;
 }
 
+// What an in-place operation does beside writing: autograd sees that a value it
+// keeps for a backward pass is no longer the one it kept.
+void written(const at::Tensor *t) {
+  if (t != nullptr && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // `given` (a borrowed reference) or a wrapped new tensor.
 PyObject *answer(PyObject *given, const at::Tensor &made) {
   if (given != Py_None) {
@@ -261,7 +267,9 @@ PyObject *rotate_store(PyObject *, PyObject *const *v, Py_ssize_t n) {
                                     code(cos.scalar_type()), rows, rotary, given->data_ptr(), q_stride, key.data_ptr(),
                                     value.data_ptr(), c.blocks, block, c.stride, call.device(), stream);
     });
-    return done(rc) ? answer(v[11], made) : nullptr;
+    if (!done(rc)) return nullptr;
+    for (const at::Tensor *t : {&key, &value, given}) written(t);
+    return answer(v[11], made);
   });
 }
 
@@ -310,7 +318,9 @@ PyObject *paged_attention(PyObject *, PyObject *const *v, Py_ssize_t n) {
                                  static_cast<float>(scale), given->data_ptr(), out_stride, static_cast<float *>(pointer(lse)),
                                  need > 0 ? workspace.data_ptr() : nullptr, need, call.device(), stream);
     });
-    return done(rc) ? answer(v[6], made) : nullptr;
+    if (!done(rc)) return nullptr;
+    for (const at::Tensor *t : {given, lse}) written(t);
+    return answer(v[6], made);
   });
 }
 
@@ -395,7 +405,9 @@ PyObject *choose(PyObject *, PyObject *const *v, Py_ssize_t n) {
                               static_cast<const uint32_t *>(pointer(allowed)), allowed_stride, floats(processed), processed_stride,
                               static_cast<int64_t *>(given->data_ptr()), append, call.device(), stream);
     });
-    return done(rc) ? answer(v[13], made) : nullptr;
+    if (!done(rc)) return nullptr;
+    for (const at::Tensor *t : {given, processed, append != 0 ? history : nullptr}) written(t);
+    return answer(v[13], made);
   });
 }
 
