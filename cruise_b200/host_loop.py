@@ -17,12 +17,14 @@ tokens, biases, a grammar mask), which the resident epoch does not take.
 
 from __future__ import annotations
 
-from typing import Callable, Sequence
+from typing import TYPE_CHECKING, Callable, Sequence
 
 import numpy as np
-import torch
 
 from .model_config import BATCH, MAX_STEPS
+
+if TYPE_CHECKING:
+    import torch
 
 FINISH_NONE, FINISH_EOS, FINISH_MAX_STEPS, FINISH_EMPTY, FINISH_ALREADY_FINISHED = 0, 1, 2, 4, 5
 
@@ -69,6 +71,8 @@ class RuledChoice:
                  repetition: float | Sequence[float] = 1.0, frequency: float | Sequence[float] = 0.0,
                  presence: float | Sequence[float] = 0.0, bias: Sequence[dict[int, float] | None] | None = None,
                  allowed: torch.Tensor | None = None) -> None:
+        import torch
+
         rows = len(prompts)
         lengths = [len(p) for p in prompts]
         if capacity < 1 or max(lengths, default=0) > capacity:
@@ -101,6 +105,8 @@ class RuledChoice:
             self.rules["bias_len"] = torch.tensor([len(e) for e in lists], dtype=torch.int32, device=cuda)
 
     def __call__(self, logits: torch.Tensor, active) -> np.ndarray:
+        import torch
+
         from . import decoder_ops
 
         flags = torch.as_tensor(np.asarray(active, dtype=np.int32), device=self.history.device)
