@@ -3,16 +3,19 @@ server (a plain C++ program over the library's C ABI) and the Python calls of
 the decoder operators (an extension module against torch's headers).
 
 ``python -m cruise_b200.build`` writes ``cruise_b200/libcruise_epoch.so``,
-``cruise_b200/cruise_epoch_server`` and ``cruise_b200/_decoder_bind.so``.  nvcc cross-compiles without a GPU, so this
-runs on any host with CUDA 12.9.
+``cruise_b200/cruise_epoch_server`` and ``cruise_b200/_decoder_bind.so``.  nvcc
+cross-compiles without a GPU, so this runs on any host with CUDA 12.9; where torch
+or the Python headers are missing, the extension module is left out.
 """
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -46,7 +49,7 @@ def _fresh(target: Path, sources: list[Path]) -> bool:
 
 def up_to_date() -> bool:
     return (_fresh(LIBRARY, SOURCES) and _fresh(SERVER, SERVER_SOURCES + [LIBRARY])
-            and _fresh(BINDING, BINDING_SOURCES))
+            and (_fresh(BINDING, BINDING_SOURCES) or not binding_possible()))
 
 
 def build_server() -> Path:
@@ -62,10 +65,14 @@ def build_server() -> Path:
     return SERVER
 
 
+def binding_possible() -> bool:
+    """Whether this host has what the Python calls are built against; callers of
+    the library in C need neither."""
+    return importlib.util.find_spec("torch") is not None and Path(sysconfig.get_paths()["include"], "Python.h").exists()
+
+
 def build_binding() -> Path:
     """The Python calls of the decoder operators (cruise_b200._decoder_bind)."""
-    import sysconfig
-
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 
@@ -100,7 +107,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         os.replace(tmp, LIBRARY)
     build_server()
     if force or not _fresh(BINDING, BINDING_SOURCES):
-        build_binding()
+        if binding_possible():
+            build_binding()
+        else:
+            print(f"{BINDING.name} not built: no torch or no Python headers here (cruise_b200.decoder_ops needs it)", file=sys.stderr)
     return LIBRARY
 
 

@@ -24,3 +24,25 @@ import numpy as np
 from cruise_b200.host_loop import first_max, host_loop_epoch, row_slot
 assert first_max(np.array([0.0, 2.0, 2.0], dtype=np.float32)) == 1
 """)
+
+
+def test_the_build_leaves_the_python_calls_out(tmp_path):
+    done = run(f"""
+from pathlib import Path
+from cruise_b200 import build
+build.BINDING = Path({str(tmp_path)!r}) / "_decoder_bind.so"
+build._fresh = lambda target, sources: target.exists()   # the library and the server are there
+compiled = []
+build.build_server = lambda: compiled.append("server")
+assert build.up_to_date()
+assert build.build() == build.LIBRARY and not compiled
+build.up_to_date = lambda: False
+assert build.build() == build.LIBRARY and compiled == ["server"] and not build.BINDING.exists()
+""")
+    assert "_decoder_bind.so not built" in done.stderr
+
+
+def test_the_build_has_the_python_calls_where_torch_is():
+    from cruise_b200 import build
+
+    assert build.binding_possible()
