@@ -519,7 +519,7 @@ static int32_t check_attention_sizes(const char *op, int32_t rows, int32_t num_h
   if (head_dim != 64 && head_dim != 128) return refuse("%s: head size %d (64 or 128)", op, head_dim);
   constexpr int kTile = kAttendWarps * kAttendKeys;
   // (the kernels count positions a few tiles past the end, and work up to a CTA's share past it, in 32 bits)
-  if (capacity < 0 || capacity > kMaxIndex - 4 * kTile) return refuse("%s: a capacity of %lld positions (below 2^31)", op, static_cast<long long>(capacity));
+  if (capacity < 0 || capacity > kMaxIndex - 4 * kTile) return refuse("%s: a capacity of %lld positions (below 2^31 - 256)", op, static_cast<long long>(capacity));
   const int64_t units = static_cast<int64_t>(num_kv_heads) * ((num_heads / num_kv_heads + 15) / 16);
   if (rows * units * (std::max<int64_t>(1, (capacity + kTile - 1) / kTile) + attend_setup(head_dim)) > kMaxIndex - 1024)
     return refuse("%s: rows x KV heads x capacity / %d passes 2^31", op, kTile);

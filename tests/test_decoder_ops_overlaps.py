@@ -71,3 +71,12 @@ def test_choose_takes_neighbours_and_a_history_it_only_reads():
                    dict(append=0, history_len=at(1) + 8), dict(repetition=at(9), presence=at(9)), dict(processed=at(0))):
         rc, why = call("cruise_decoder_choose", {**CHOOSE, **EVERY, **change})
         assert rc > 0, why   # no device: past every check
+
+
+def test_the_capacity_s_limit_is_the_one_that_is_named():
+    from cruise_b200 import _lib
+
+    workspace = _lib.load().cruise_decoder_attention_workspace
+    assert workspace(1, 1, 1, 64, 2 ** 31 - 257, 0) > 0
+    assert workspace(1, 1, 1, 64, 2 ** 31 - 256, 0) == -1
+    assert "below 2^31 - 256" in _lib.load().cruise_decoder_last_error().decode()
