@@ -91,3 +91,20 @@ def test_penalties_that_are_not_finite_act_on_the_tokens_they_are_for():
         assert torch.equal(room[r][untouched & allowed], case["logits"][r][untouched & allowed])
         if r in (0, 3):   # an infinite penalty bans what was said
             assert (room[r][output] == -math.inf).all() and int(token[r]) not in output.tolist() and token[r] >= 0
+
+
+@pytest.mark.parametrize("rows, vocab, cap", [(70, 152064, 13001), (40, 100003, 32768), (3, 390000, 20000)])
+def test_histories_far_wider_than_what_they_hold(rows, vocab, cap):
+    """Tensors so wide that a row takes sixteen CTAs however many rows there are;
+    their rows hold a few tokens, some hold all the tensor has."""
+    case = choose_case(rows, vocab, BF16, cap=cap, seed=63)
+    case["history_len"][:] = torch.arange(rows, device="cuda") % 50
+    case["history_len"][rows - 1] = cap - 1
+    case["prompt_len"][:] = case["history_len"] // 2
+    token = check_choose(case, processed=False, append=False)
+    tight = dict(case)
+    narrow = int(case["history_len"][:-1].max())
+    tight["history"] = case["history"][:, :max(narrow, 1)].contiguous()
+    from cruise_b200.decoder_ops import choose
+
+    assert torch.equal(choose(**tight)[:-1], token[:-1])

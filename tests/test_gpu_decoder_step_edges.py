@@ -1,12 +1,14 @@
 """The paged decoder step (cruise_decoder_step_paged) at its edges: refusals of
-the C entry before anything is launched."""
+the C entry before anything is launched, rows it leaves out, wide tables, large
+batches, tables and logits in other forms, other streams."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
-from test_gpu_decoder_step_paged import GEOMETRY, _pair
+from scenario import rel_err_rows
+from test_gpu_decoder_step_paged import GEOMETRY, TOL, _pair, _tables
 
 pytestmark = pytest.mark.gpu
 
@@ -157,3 +159,87 @@ def test_the_same_arrays_are_taken(engine):
     rc, why = step(engine, t)
     assert rc == 0, why
     assert t["logits"].any() and t["key"].any()
+
+
+# ---- what a decode loop does with the step ---------------------------------------------------
+
+
+def batch(rows, width, seed, used=4):
+    """Rows of up to ``used`` blocks each, in tables ``width`` blocks wide."""
+    gen = torch.Generator().manual_seed(seed)
+    shape = (GEOMETRY["num_layers"], rows * used, BLOCK, GEOMETRY["num_kv_heads"], GEOMETRY["head_dim"])
+    key, value = (torch.randn(shape, generator=gen).to(torch.bfloat16).cuda() for _ in range(2))
+    table = torch.full((rows, width), -1, dtype=torch.int32)
+    table[:, :used] = torch.randperm(rows * used, generator=gen).int().reshape(rows, used)
+    token = torch.randint(0, GEOMETRY["vocab"], (rows,), generator=gen)
+    position = torch.randint(0, used * BLOCK, (rows,), generator=gen)
+    return token.cuda(), position.cuda(), table.cuda(), key, value
+
+
+def close(a, b):
+    assert float(rel_err_rows(a.float().cpu().flatten(1), b.float().cpu().flatten(1)).max()) <= TOL
+
+
+def workspace(engine, rows, width):
+    return engine.lib.cruise_decoder_attention_workspace(rows, GEOMETRY["num_heads"], GEOMETRY["num_kv_heads"],
+                                                         GEOMETRY["head_dim"], width * BLOCK, 0)
+
+
+def test_wide_tables_take_the_split_form(engine):
+    """Tables for 32000 positions: the engine's attention is split over all CTAs and
+    joined, with a workspace of the engine's that later calls share."""
+    assert workspace(engine, 4, 4) == 0 and workspace(engine, 4, 2000) == workspace(engine, 64, 4000) > 0
+    for rows, width in ((4, 2000), (64, 4000), (3, 2000), (4, 2000)):
+        token, position, table, key, value = batch(rows, width, seed=rows)
+        narrow_key, narrow_value = key.clone(), value.clone()
+        narrow = engine.decoder_step_paged(token, position, table[:, :4].contiguous(), narrow_key, narrow_value)
+        wide = engine.decoder_step_paged(token, position, table, key, value)
+        close(wide, narrow)
+        for a, b in ((key, narrow_key), (value, narrow_value)):
+            close(a.flatten(0, 3), b.flatten(0, 3))
+
+
+@pytest.mark.parametrize("rows", [129, 200, 256])
+def test_batches_past_one_token_tile(engine, rows):
+    token, position, table, key, value = batch(rows, 4, seed=rows)
+    k1, v1 = key.clone(), value.clone()
+    together = engine.decoder_step_paged(token, position, table, key, value)
+    for r in (0, rows // 2, rows - 1):
+        one = engine.decoder_step_paged(token[r:r + 1], position[r:r + 1], table[r:r + 1], k1, v1)
+        close(one, together[r:r + 1])
+
+
+def test_fp32_tables_of_the_same_values_give_the_same_step(engine):
+    token, position, table, key, value = batch(5, 4, seed=80)
+    cos, sin = _tables(engine, BLOCK * 4)
+    assert cos.dtype == torch.bfloat16
+    k1, v1 = key.clone(), value.clone()
+    want = engine.decoder_step_paged(token, position, table, k1, v1, cos, sin)
+    got = engine.decoder_step_paged(token, position, table, key, value, cos.float(), sin.float())
+    assert torch.equal(got, want) and torch.equal(key, k1) and torch.equal(value, v1)
+
+
+def test_logits_inside_a_wider_tensor(engine):
+    token, position, table, key, value = batch(5, 4, seed=81)
+    want = engine.decoder_step_paged(token, position, table, key.clone(), value.clone())
+    room = torch.full((5, GEOMETRY["vocab"] + 24), 7.0, dtype=torch.bfloat16, device="cuda")
+    got = engine.decoder_step_paged(token, position, table, key, value, logits_out=room[:, 8:-16])
+    assert got.data_ptr() == room[:, 8:].data_ptr() and torch.equal(got, want)
+    assert (room[:, :8] == 7).all() and (room[:, -16:] == 7).all()
+
+
+def test_the_step_follows_the_current_stream(engine):
+    """Inputs written late on another stream, and a reader on it right after."""
+    token, position, table, key, value = batch(6, 4, seed=82)
+    k1, v1 = key.clone(), value.clone()
+    want = engine.decoder_step_paged(token, position, table, k1, v1)
+    late = [torch.zeros_like(token), torch.full_like(position, -1), torch.zeros_like(key)]
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(20_000_000)
+        for to, source in zip(late, (token, position, key)):
+            to.copy_(source)
+        got = engine.decoder_step_paged(late[0], late[1], table, late[2], value).clone()
+    stream.synchronize()
+    assert torch.equal(got, want) and torch.equal(late[2], k1) and torch.equal(value, v1)
