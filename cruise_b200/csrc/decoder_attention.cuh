@@ -20,7 +20,7 @@
 // 1% of the long cases.
 //
 // What bounds it is the cache's bytes: a key and its value, 4 d bytes, take 4 d
-// operations for each of the group's heads, far below the tensor pipe (8% of
+// operations for each of the group's heads, far below the tensor pipe (13% of
 // its cycles at 64 ragged rows).  So the products are the warp-wide ones, whose
 // operands a warp takes from its own ring as they arrive, 16 keys a step, with
 // no barrier between warps until the unit's end; larger tiles would only wait
@@ -29,7 +29,7 @@
 // the join); 64 ragged rows of up to 16384 in pages of 16, head size 64, 46 us
 // (75%: units of a few steps, and two steps of copies in flight per warp).  Few
 // and short units are bounded by the chain of start, first loads, products and
-// merge: 4 rows of 256 4.3 us, 4 of 16 2.6.
+// merge: 4 rows of 256 4.4 us, 4 of 16 2.6.
 //
 // Which CTAs take a unit (a row and a KV head, at most 16 query heads):
 //   split:   all CTAs share all tiles evenly, whatever the rows' lengths, and a

@@ -24,8 +24,8 @@
 // rule and the processed logits written take 74 us, 66% of the copy bandwidth (the
 // stream alone 57; then the marked tokens' values and second looks, while little
 // is in flight).  For few rows the chain of the marked tokens' steps (clear, mark,
-// rank, count, value, compare): 4.1 us for one row of 4096, 5.5 for 4 of 152064,
-// 8.0 for 64 of 50257 with 1000 entries each.  Two kernels, one for the marked
+// rank, count, value, compare): 4.2 us for one row of 4096, 5.6 for 4 of 152064,
+// 8.1 for 64 of 50257 with 1000 entries each.  Two kernels, one for the marked
 // tokens, took 126 us for the 256 rows; one CTA's warps doing first the one and
 // then the other 82.
 #pragma once

@@ -192,6 +192,8 @@ AttentionShape attention_shape(int32_t rows, int32_t nq, int32_t nkv, int32_t d,
   //   8 x 16: one warp 2.6, four 2.8, eight 3.6; 8 x 64: 4.3, 2.8, 3.7
   //   300 x 64: one 5.1, four 5.4; 300 x 128: 7.5, 6.4; 1200 x 256: 23.0, 28.6
   //   (head size 64, whose four-warp CTAs are smaller: 600 x 128: 6.7, 5.7; 1200 x 128: 8.2, 9.3)
+  // (Short rows in a wide table are taken for long ones: 4 rows of 256 4.5 us, in a table
+  // for 131072 positions 8.1; 64 of up to 500 8.5 and 11.2.)
   if (capacity <= kAttendKeys || (units * d >= 512 * capacity && capacity <= 512)) {
     s.warps = 1;
     return s;
@@ -339,6 +341,9 @@ cudaError_t choose_typed(const ChooseArgs &a, int device, cudaStream_t stream) {
   // two to an SM, the first takes 1.3 and the stream 1.6 times as long.  One row
   // of 152064 with 1000 entries: 6.0 us with 16 CTAs, 7.6 with four, 14.3 with one;
   // 17 rows: 12.9, 8.0, 16.3; 64 rows: 36 with 16, 12.6 with four, 26 with one.
+  // The entries are the tensors' widths, for the lengths are on the device: where
+  // these are far smaller, a wide history still costs a cluster's room (64 rows of
+  // 152064 with 1000 tokens: 10.8 us in a history of 1024, 13.0 of 8192, 31.9 of 32768).
   int best = 0;
   bool alone = false;
   double least = 0;

@@ -58,7 +58,8 @@ class RuledChoice:
     grow with each choice.
 
     ``prompts``: the rows' tokens so far (they count for ``repetition``);
-    ``capacity``: the longest history.  ``repetition``, ``frequency``,
+    ``capacity``: the longest history (the wider, the slower where rows are many:
+    :func:`~cruise_b200.decoder_ops.choose` is planned by it).  ``repetition``, ``frequency``,
     ``presence``: a number, or one per row.  ``bias``: per row a dict of token to
     bias, or None.  ``allowed``: int32 bit masks [rows, ceil(vocab / 32)] on the
     device (replace or rewrite them between steps as a grammar advances).

@@ -60,7 +60,8 @@ int32_t cruise_decoder_rotate_store(
  * apart) = softmax(scale q K^T) V, lse (may be NULL) [rows][num_heads] fp32 the
  * natural logarithm of the softmax's sum.  Positions whose block lies outside
  * [0, num_blocks) are left out; a row with no position left gets zeros and
- * lse -inf.  The values of table entries past a row's length do not matter.
+ * lse -inf.  The values of table entries past a row's length do not matter; the
+ * launch is planned by table_width, so one close to the lengths is faster.
  * workspace: cruise_decoder_attention_workspace() bytes, 16-byte aligned, not
  * shared by calls that may overlap (its contents do not matter between calls);
  * NULL where that returns 0.  Other pointers 16-byte aligned (block_table,
@@ -106,10 +107,11 @@ int64_t cruise_decoder_attention_workspace(int32_t rows, int32_t num_heads,
  * processed value is NaN or +inf.  processed (may be NULL) [rows][vocab] fp32,
  * rows processed_stride apart: the x; it may be the logits themselves (fp32,
  * same stride), else must not overlap them.  token, processed and, with append,
- * history must not overlap one another or the other inputs.  append: token[r] >= 0 is written to
- * history[r][history_len[r]] where that is inside history_width (history_len
- * itself is the caller's to advance).  4-byte alignment suffices (logits: their
- * own size).  vocab at most 2^20; fewer than 2^30 history and bias entries
+ * history must not overlap one another or the other inputs.  append: token[r] >= 0
+ * is written to history[r][history_len[r]] where that is inside history_width
+ * (history_len itself is the caller's to advance).  4-byte alignment suffices (logits: their
+ * own size).  The launch is planned by history_width and bias_width, so a width
+ * close to the lengths is faster.  vocab at most 2^20; fewer than 2^30 history and bias entries
  * together, beyond 390000 logits at most 20000. */
 int32_t cruise_decoder_choose(
     const void *logits, int64_t logits_stride, int32_t rows, int32_t vocab,
