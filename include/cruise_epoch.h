@@ -297,7 +297,8 @@ int32_t cruise_decoder_step(void *engine, const int64_t *token,
  * position lies past its block table, is inactive too; the logits of inactive
  * rows must not be used.  A row whose position has no row in the rotation tables,
  * or a table entry that is no block of the cache, is left out like an inactive
- * one, and the call returns -5 once the step has completed for the others.  Two
+ * one, and the call returns -5 once the step has completed for the others.
+ * Earlier positions whose entry is no block are left out of a row's attention.  Two
  * rows must not share a slot, and the caches and the logits must not overlap one
  * another or the inputs.  rows at most 4 block_size of the engine.
  * logits: bf16 [rows][vocab], rows logits_stride elements apart (the decoder's
