@@ -283,33 +283,34 @@ int32_t cruise_decoder_step(void *engine, const int64_t *token,
                             void *value_cache, const uint8_t *tiling,
                             float *logits_out, int64_t *next_position_out);
 
-/* One decoder step of any number of rows over caller-held paged caches of any
- * length, layer by layer: the engine's projections around the decoder
- * operators of cruise_decoder.h (rotate_store and paged_attention), where the
- * resident kernel holds four rows of blocks_per_row blocks.  Every array is
- * device memory on the engine's device: token i64[rows] and position i64[rows]
- * (negative: the row is inactive), caches bf16 [layers][num_blocks][block_size]
- * [kv_heads][head_dim] (16-byte aligned, updated in place at each position's
- * slot), block_table i32 [rows][table_width] (rows table_stride entries apart),
- * rope_cos / rope_sin [rope_rows][head_dim] of rope_dtype 0 (bf16) or 2 (fp32),
- * (16-byte aligned), or both NULL for the engine's own tables (the positions of its resident rows:
- * blocks_per_row * block_size).  A row whose token does not exist, or whose
- * position lies past its block table, is inactive too; the logits of inactive
- * rows must not be used.  A row whose position has no row in the rotation tables,
- * or a table entry that is no block of the cache, is left out like an inactive
- * one, and the call returns -5 once the step has completed for the others.
- * Earlier positions whose entry is no block are left out of a row's attention.  Two
- * rows must not share a slot, and the caches and the logits must not overlap one
- * another or the inputs.  rows at most 4 block_size of the engine.
+/* One decoder step of up to 4 block_size rows (the engine's) over caller-held
+ * paged caches of any length, layer by layer: the engine's projections around
+ * the decoder operators of cruise_decoder.h (rotate_store and paged_attention),
+ * where the resident kernel holds four rows of blocks_per_row blocks.  Every
+ * array is device memory on the engine's device: token i64[rows] and position
+ * i64[rows] (negative: the row is inactive), caches bf16 [layers][num_blocks]
+ * [block_size][kv_heads][head_dim] (16-byte aligned, updated in place at each
+ * position's slot), block_table i32 [rows][table_width] (rows table_stride
+ * entries apart), rope_cos / rope_sin [rope_rows][head_dim] of rope_dtype 0
+ * (bf16) or 2 (fp32), 16-byte aligned, or both NULL for the engine's own tables
+ * (the positions of its resident rows: blocks_per_row * block_size).
+ * A row whose token does not exist, or whose position lies past its block
+ * table, is inactive too; the logits of inactive rows must not be used.  A row
+ * whose position has no row in the rotation tables, or a table entry that is no
+ * block of the cache, is left out like an inactive one, and the call returns -5
+ * once the step has completed for the others.  Earlier positions whose entry is
+ * no block are left out of a row's attention.  Two rows must not share a slot,
+ * and the caches and the logits must not overlap one another or the inputs.
  * logits: bf16 [rows][vocab], rows logits_stride elements apart (the decoder's
  * rounding: cruise_decoder_step gives the same values as f32).  Rounds where the
  * decoder does, but for the attention's scores and probabilities and the
- * rotation, which stay in fp32.
+ * rotation, which keep more bits (cruise_decoder.h).
  * Waits for what `stream` holds, and returns when the step has completed (so
  * a capturing stream is refused).
  * Returns 0, -1 for invalid arguments, -2 when a projection could not be
  * launched, -3 when a device-side wait gave up, -4 for a tensor-parallel
- * engine, -5 when rows were left out (the message names the first), or a CUDA error code; cruise_epoch_last_error explains them. */
+ * engine, -5 when rows were left out (the message names the first), or a CUDA
+ * error code; cruise_epoch_last_error explains them. */
 int32_t cruise_decoder_step_paged(
     void *engine, int32_t rows, const int64_t *token, const int64_t *position,
     void *key_cache, void *value_cache, int64_t num_blocks, int32_t block_size,
